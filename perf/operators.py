@@ -501,7 +501,10 @@ def _pages_own(state):
         begun = tables.clone(), lens.clone(), refs.clone()
         plan.release(tables, lens, refs, state["rows"])
         return cache, state["fresh"], begun, tables, lens, refs
-    plan.compact(cache, tables, refs, state["tables_out"], state["refs_out"], state["remap"], state["live"])
+    if "workspace" not in state:
+        state["workspace"] = torch.empty(plan.workspace_size(), dtype=torch.uint8, device=DEV)
+    plan.compact(cache, tables, refs, state["tables_out"], state["refs_out"], state["remap"], state["live"],
+                 workspace=state["workspace"])
     return cache, state["tables_out"], state["refs_out"], state["remap"], state["live"]
 
 
