@@ -1,0 +1,181 @@
+// kv4_attention.hpp -- what the attention kernels over 4-bit pages share: the
+// arguments, which tokens a block of rows sees, and how the work is cut.
+//
+//   o = softmax(scale q k^T + mask) v
+//
+// A sequence's new tokens are its last ones: token i of n stands at position
+// len - n + i.  A row (a token and a head) sees the positions up to its own
+// (all of the sequence without `causal`) and, with a window w, the last w of
+// those.  A row that sees nothing gives zeros.  Rows of one kv head are taken
+// together: row r is token r / ratio and head r % ratio of the group.
+#pragma once
+
+#include "kv4.hpp"
+
+namespace bk {
+namespace kv4 {
+
+struct AttnArgs {
+    const void *q;
+    void *out;
+    const uint8_t *cache;
+    const int32_t *tables, *lens, *cu_q;
+    int64_t q_token, q_head, out_token, out_head, table_stride, num_pages;
+    int64_t part;              // bytes from `split` to the partial results
+    char *split;               // workspace: int2 per item, then m and l, then O of each part
+    int num_seqs, total_q, hq, hk, ratio, max_pages, ps, ps_shift, causal, window;
+    int row_blocks;            // blocks of rows of a sequence
+    int items;                 // num_seqs * row_blocks
+    int slots;                 // workgroups that the parts are made for; 0: nothing is split
+    int min_tiles;             // tiles of 16 tokens that a part has at least
+    float scale;               // times log2(e)
+};
+
+// A block of rows and the tokens [lo, hi) that any of them sees.
+struct Item {
+    int seq, q0, first, rows, base, len, lo, hi;
+};
+
+__device__ __forceinline__ Item item_of(const AttnArgs &a, int item, int block) {
+    Item s;
+    s.seq = item / a.row_blocks;
+    int q0 = s.seq, n = 1;
+    if (a.cu_q) {
+        q0 = a.cu_q[s.seq];
+        n = a.cu_q[s.seq + 1] - q0;
+    }
+    if (q0 < 0 || n < 0 || n > a.total_q - q0) n = 0;
+    const int len = a.lens[s.seq];
+    const int64_t room = (int64_t)a.max_pages << a.ps_shift;
+    s.q0 = q0;
+    s.base = len - n;
+    s.len = (int)(len < room ? len : room);
+    s.first = item % a.row_blocks * block;
+    s.rows = min(block, n * a.ratio - s.first);
+    s.lo = s.hi = 0;
+    if (s.rows > 0) {
+        const int i0 = s.first / a.ratio, i1 = (s.first + s.rows - 1) / a.ratio;
+        s.hi = max(0, a.causal ? min(s.len, s.base + i1 + 1) : s.len);
+        s.lo = a.window ? max(0, s.base + i0 - a.window + 1) : 0;
+    }
+    return s;
+}
+
+__device__ __forceinline__ int tiles_of(const Item &s) { return s.hi > s.lo ? (s.hi + 15) / 16 - s.lo / 16 : 0; }
+
+// The tokens that a row sees: [lo, hi).
+__device__ __forceinline__ void row_span(const AttnArgs &a, const Item &s, int r, int &lo, int &hi) {
+    const int pos = s.base + (s.first + r) / a.ratio;
+    const bool in = r < s.rows;
+    hi = in ? (a.causal ? min(s.len, pos + 1) : s.len) : 0;
+    lo = in && a.window ? max(0, pos - a.window + 1) : 0;
+}
+
+__device__ __forceinline__ int wave_sum(int x) {
+#pragma unroll
+    for (int m = 1; m < 64; m *= 2) x += __shfl_xor(x, m, 64);
+    return x;
+}
+
+// A part of an item: tiles [t0, t1) of 16 tokens.  `parts` parts have the item,
+// the first of them is part `begin` of all.
+struct Part {
+    int item, t0, t1, parts, begin;
+};
+
+// Part `index` of all, worked out from the lengths by one wave: all items
+// together are cut into about slots / hk parts of one size, so that the
+// longest sequence does not hold up the launch.  Items of one wave's width
+// cost one pass over the lengths.  item < 0: there is no such part.
+__device__ __forceinline__ Part find_part(const AttnArgs &a, int block, int index) {
+    const int lane = threadIdx.x & 63;
+    int total = 0;
+    for (int i0 = 0; i0 < a.items; i0 += 64) {
+        const int i = i0 + lane;
+        total += wave_sum(i < a.items ? tiles_of(item_of(a, i, block)) : 0);
+    }
+    const int per = max(a.min_tiles, (int)(((int64_t)total * a.hk + a.slots - 1) / a.slots));
+    Part p{-1, 0, 0, 0, 0};
+    int begin = 0;
+    for (int i0 = 0; i0 < a.items; i0 += 64) {
+        const int i = i0 + lane;
+        int n = 0, tiles = 0, lo = 0;
+        if (i < a.items) {
+            const Item s = item_of(a, i, block);
+            tiles = tiles_of(s);
+            lo = s.lo / 16;
+            n = s.rows > 0 ? max(1, (tiles + per - 1) / per) : 0;
+        }
+        int sum = n;
+#pragma unroll
+        for (int d = 1; d < 64; d *= 2) {
+            const int o = __shfl_up(sum, d, 64);
+            if (lane >= d) sum += o;
+        }
+        const int mine = begin + sum - n;
+        const uint64_t hit = __ballot(index >= mine && index < mine + n);
+        if (hit) {
+            const int src = __builtin_ctzll(hit);
+            p.item = i0 + src;
+            p.parts = __shfl(n, src, 64);
+            p.begin = __shfl(mine, src, 64);
+            tiles = __shfl(tiles, src, 64);
+            lo = __shfl(lo, src, 64);
+            // equal parts of the item
+            const int each = (tiles + p.parts - 1) / p.parts, k = index - p.begin;
+            p.t0 = lo + min(tiles, k * each);
+            p.t1 = lo + min(tiles, (k + 1) * each);
+            return p;
+        }
+        begin += __shfl(sum, 63, 64);
+    }
+    return p;
+}
+
+template <typename T>
+__device__ __forceinline__ v4f mfma_pv(const v4i &a, const v4i &b, const v4f &c);
+template <>
+__device__ __forceinline__ v4f mfma_pv<Bf16>(const v4i &a, const v4i &b, const v4f &c) {
+    return mfma16x16x32_h<true>(a, b, c);
+}
+template <>
+__device__ __forceinline__ v4f mfma_pv<F16>(const v4i &a, const v4i &b, const v4f &c) {
+    return mfma16x16x32_h<false>(a, b, c);
+}
+
+typedef _Float16 f16x2_t __attribute__((ext_vector_type(2)));
+
+// Byte `sel` of w, two codes, as a pair of elements under `scale` (exact for
+// every scale that kv4_append writes; f16 rounds scales below 2^-23).
+template <typename T>
+__device__ __forceinline__ uint32_t pair_of(uint32_t w, float scale, int sel) {
+    if constexpr (__is_same(T, Bf16)) {
+        switch (sel) {
+            case 0: return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, 0));
+            case 1: return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, 1));
+            case 2: return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, 2));
+            default: return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, 3));
+        }
+    } else {
+        switch (sel) {
+            case 0: return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, scale, 0));
+            case 1: return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, scale, 1));
+            case 2: return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, scale, 2));
+            default: return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, scale, 3));
+        }
+    }
+}
+
+template <typename T>
+__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
+    if constexpr (__is_same(T, Bf16)) {
+        return f32x2_to_bf16x2(lo, hi);
+    } else {
+        return (uint32_t)f32_to_f16_rne(lo) | (uint32_t)f32_to_f16_rne(hi) << 16;
+    }
+}
+
+__device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
+
+}  // namespace kv4
+}  // namespace bk

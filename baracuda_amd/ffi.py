@@ -135,6 +135,28 @@ _sig("baracuda_te_recipe_update_can_implement", i32, vp, vp, vp, i32, i32, i32)
 _sig("baracuda_te_recipe_init_run", i32, vp, vp, vp, i32, vp)
 _sig("baracuda_te_recipe_init_can_implement", i32, vp, vp, vp, i32)
 
+_ROT = (vp, vp, vp, vp, vp, i64, vp)          # weights, positions, cosine, sine, table rows, pair axis
+_sig("baracuda_kernels_qk_norm_rope_gfx950_run", i32, i64, i32, i32, i32, i32, i32, i32, i32, C.c_double,
+     *(vp, i64, i64) * 4, *_ROT, vp)
+_sig("baracuda_kernels_qk_norm_rope_gfx950_can_implement", i32, i64, i32, i32, i32, i32, i32, i32)
+_sig("baracuda_kernels_kv4_append_gfx950_run", i32, i64, i32, i32, i32, i32, i32, i32, i32, C.c_double, i32, i64,
+     *(vp, i64, i64) * 4, vp, vp, *_ROT, vp)
+_sig("baracuda_kernels_kv4_append_gfx950_can_implement", i32, i64, i32, i32, i32, i32, i32, i32, i32, i64)
+_sig("baracuda_kernels_kv4_read_gfx950_run", i32, i64, i32, i32, i32, i32, i64, vp, vp, *(vp, i64, i64) * 2, vp)
+_sig("baracuda_kernels_kv4_read_gfx950_can_implement", i32, i64, i32, i32, i32, i32, i64)
+_KV4_ATTN = (i32, i32, i32, i64, i32, i32, i32, i32, i64, i32, i32, i32, i32, f32)
+_sig("baracuda_kernels_kv4_attention_gfx950_run", i32, *_KV4_ATTN, vp, i64, i64, vp, vp, i64, vp, vp, vp, i64, i64,
+     vp, sz, vp)
+_sig("baracuda_kernels_kv4_attention_gfx950_workspace_size", sz, i32, i32, i64, i32, i32, i32, i32)
+_sig("baracuda_kernels_kv4_attention_gfx950_can_implement", i32, *_KV4_ATTN)
+_KV_PAGES = (i32, i64, i64, i32, i32, i32)
+_sig("baracuda_kernels_kv_pages_copy_gfx950_run", i32, i32, i64, i64, i64, vp, vp, vp, vp)
+_sig("baracuda_kernels_kv_pages_fork_gfx950_run", i32, *_KV_PAGES, i32, vp, vp, vp, vp, vp, vp, vp, vp)
+_sig("baracuda_kernels_kv_pages_release_gfx950_run", i32, i64, i32, i32, i32, vp, vp, vp, vp, vp)
+_sig("baracuda_kernels_kv_pages_compact_gfx950_run", i32, *_KV_PAGES, vp, vp, vp, vp, vp, vp, vp, vp, sz, vp)
+_sig("baracuda_kernels_kv_pages_gfx950_workspace_size", sz, *_KV_PAGES)
+_sig("baracuda_kernels_kv_pages_gfx950_can_implement", i32, *_KV_PAGES)
+
 SYMBOLS = tuple(_SIGS)
 
 _lib = None

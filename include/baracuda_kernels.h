@@ -12,7 +12,8 @@
  *     captured into a hipGraph;
  *   - `stream` is a hipStream_t passed as void* (NULL = default stream);
  *   - strides and leading dimensions are in elements;
- *   - workspace is never required: every _workspace_size returns 0 except
+ *   - workspace is never required, but for the 4-bit cache's attention and
+ *     page compaction: every other _workspace_size returns 0 except
  *     the u8 RRR family's, gemv_dense_m1's (large shapes) and the int8 RCR
  *     SKUs' (s8 / i32 / W8A8 bf16 out and the bias family, when the last
  *     round of 256 x 256 tiles on the 256 CUs is at most half full and the
@@ -23,8 +24,7 @@
  *     optional workspace (when given at least that size, 256- / 16-byte
  *     aligned; contents on entry do not matter) selects a faster path: the
  *     u8 pre-pass, the dense GEMV's split-K, the int8 tail round split along
- *     K (two launches, bit-identical output).  Without it every entry point
- *     runs as-is.
+ *X
  *
  * Each declaration cites the reference entry point it replaces
  * (paths relative to the baracuda repository root).
@@ -550,6 +550,127 @@ int32_t baracuda_kernels_moe_s8_grouped_i32_gfx950_run(
     int32_t num_experts, int32_t topk, int32_t size_m, int32_t size_n, int32_t size_k, void *stream);
 int32_t baracuda_kernels_moe_s8_grouped_i32_gfx950_can_implement(
     int32_t num_experts, int32_t topk, int32_t size_m, int32_t size_n, int32_t size_k);
+
+/* ======================= 4-bit key-value cache ===========================
+ * No counterpart in the reference: the step between the QKV projection and
+ * attention, a cache of keys and values in pages of 4-bit codes, attention over
+ * it, and the pages' management.  `element`: 0 f32, 1 f16, 2 bf16.
+ *
+ * The cache is uint8 [num_pages, num_kv_heads, page_size * (D + D / 16)], 16-byte
+ * aligned, two codes a byte, the lower index in the lower four bits; a code is
+ * sign, two exponent bits, one mantissa bit (0, 0.5, 1, 1.5, 2, 3, 4, 6).  32
+ * consecutive values of a head share a scale 2^(byte - 127); byte 255 marks a
+ * group that held an infinity or a NaN and reads as NaN.  The bytes of a page
+ * and a head: K codes [PS][D/2], V codes [PS/4][16][4][D/32], K scales
+ * [PS][D/32], V scales [PS/4][D/32][4].  page_size: a power of two in 16..1024;
+ * D: 64, 128 or 256.  A slot is page * page_size + the token's place in it.
+ * Strides are in elements; the last dimension is dense. */
+
+/* y = x w / sqrt(mean(x^2) + eps) for each head of Q and K (weights NULL: no
+ * norm), then the rotation of the first rope_dim values in pairs (i, i + rope/2),
+ * interleaved != 0: (2i, 2i + 1).  cosine, sine: f32 [table_rows, rope_dim / 2];
+ * positions int32 [axes, tokens]; pair_axis int32 [rope_dim / 2], the axis of
+ * each pair (axes > 1).  A position or axis out of range gives NaN.  head_dim and
+ * rope_dim are multiples of 16 up to 256 (rope_dim may be 0).  Outputs may be the
+ * inputs themselves. */
+int32_t baracuda_kernels_qk_norm_rope_gfx950_run(
+    int64_t tokens, int32_t num_heads, int32_t num_kv_heads, int32_t head_dim, int32_t rope_dim, int32_t axes,
+    int32_t interleaved, int32_t element, double eps, const void *q, int64_t q_token_stride, int64_t q_head_stride,
+    const void *k, int64_t k_token_stride, int64_t k_head_stride, void *q_out, int64_t q_out_token_stride,
+    int64_t q_out_head_stride, void *k_out, int64_t k_out_token_stride, int64_t k_out_head_stride, const void *q_weight,
+    const void *k_weight, const int32_t *positions, const float *cosine, const float *sine, int64_t table_rows,
+    const int32_t *pair_axis, void *stream);
+int32_t baracuda_kernels_qk_norm_rope_gfx950_can_implement(
+    int64_t tokens, int32_t num_heads, int32_t num_kv_heads, int32_t head_dim, int32_t rope_dim, int32_t axes,
+    int32_t element);
+
+/* The same for Q, and K (norm and rotation, rounded to the element's type) and V
+ * into the cache: the scale is the power of two that brings the group's largest
+ * magnitude below 7, codes are the nearest, ties to the even code.  A slot
+ * outside the cache is not written; two tokens of one slot are an error of the
+ * caller.  f16 and bf16.  num_heads 0: no Q. */
+int32_t baracuda_kernels_kv4_append_gfx950_run(
+    int64_t tokens, int32_t num_heads, int32_t num_kv_heads, int32_t head_dim, int32_t rope_dim, int32_t axes,
+    int32_t interleaved, int32_t element, double eps, int32_t page_size, int64_t num_pages, const void *q,
+    int64_t q_token_stride, int64_t q_head_stride, const void *k, int64_t k_token_stride, int64_t k_head_stride,
+    const void *v, int64_t v_token_stride, int64_t v_head_stride, void *q_out, int64_t q_out_token_stride,
+    int64_t q_out_head_stride, void *cache, const int64_t *slots, const void *q_weight, const void *k_weight,
+    const int32_t *positions, const float *cosine, const float *sine, int64_t table_rows, const int32_t *pair_axis,
+    void *stream);
+int32_t baracuda_kernels_kv4_append_gfx950_can_implement(
+    int64_t tokens, int32_t num_heads, int32_t num_kv_heads, int32_t head_dim, int32_t rope_dim, int32_t axes,
+    int32_t element, int32_t page_size, int64_t num_pages);
+
+/* k_out, v_out [tokens, num_kv_heads, D]: the values that the slots stand for;
+ * zeros for a slot outside the cache. */
+int32_t baracuda_kernels_kv4_read_gfx950_run(
+    int64_t tokens, int32_t num_kv_heads, int32_t head_dim, int32_t element, int32_t page_size, int64_t num_pages,
+    const void *cache, const int64_t *slots, void *k_out, int64_t k_token_stride, int64_t k_head_stride, void *v_out,
+    int64_t v_token_stride, int64_t v_head_stride, void *stream);
+int32_t baracuda_kernels_kv4_read_gfx950_can_implement(
+    int64_t tokens, int32_t num_kv_heads, int32_t head_dim, int32_t element, int32_t page_size, int64_t num_pages);
+
+/* out = softmax(scale q K^T + mask) V over the pages of each sequence.  q, out
+ * [total_q, num_heads, D]; cu_q int32 [num_seqs + 1], the first row of each
+ * sequence (NULL: one row each); kv_lens int32 [num_seqs], the tokens in the
+ * cache, a sequence's new ones being the last of them; tables int32 [num_seqs,
+ * max_pages] (table_stride), a sequence's pages in order.  max_q and max_kv are
+ * what the host knows of the lengths: rows past max_q of a sequence are not
+ * computed, max_kv only decides how the work is cut.  With `causal` a row sees
+ * the positions up to its own, with window > 0 the last `window` of those; a row
+ * that sees nothing gives zeros.  An entry outside the cache stands for tokens
+ * that no row sees.  f16 and bf16; an f16 cache is one that f16 was appended to.
+ * The workspace (16-byte aligned) is required where its size is not 0. */
+int32_t baracuda_kernels_kv4_attention_gfx950_run(
+    int32_t num_seqs, int32_t total_q, int32_t max_q, int64_t max_kv, int32_t num_heads, int32_t num_kv_heads,
+    int32_t head_dim, int32_t page_size, int64_t num_pages, int32_t max_pages, int32_t element, int32_t causal,
+    int32_t window, float scale, const void *q, int64_t q_token_stride, int64_t q_head_stride, const void *cache,
+    const int32_t *tables, int64_t table_stride, const int32_t *kv_lens, const int32_t *cu_q, void *out,
+    int64_t out_token_stride, int64_t out_head_stride, void *workspace, size_t workspace_bytes, void *stream);
+size_t baracuda_kernels_kv4_attention_gfx950_workspace_size(int32_t num_seqs, int32_t max_q, int64_t max_kv,
+                                                            int32_t num_heads, int32_t num_kv_heads, int32_t head_dim,
+                                                            int32_t window);
+int32_t baracuda_kernels_kv4_attention_gfx950_can_implement(
+    int32_t num_seqs, int32_t total_q, int32_t max_q, int64_t max_kv, int32_t num_heads, int32_t num_kv_heads,
+    int32_t head_dim, int32_t page_size, int64_t num_pages, int32_t max_pages, int32_t element, int32_t causal,
+    int32_t window, float scale);
+
+/* Pages of a cache [layers, num_pages, page_bytes] of any contents; one table
+ * serves all layers.  tables int32 [rows, max_pages] (-1: no page), lens int32
+ * [rows], refs int32 [num_pages]: how many rows hold a page, 0: free.
+ *
+ * copy: page src[i] to page dst[i] in every layer, i < count; no destination is
+ * a source or named twice.  A pair outside the cache is left out. */
+int32_t baracuda_kernels_kv_pages_copy_gfx950_run(int32_t layers, int64_t num_pages, int64_t page_bytes,
+                                                  int64_t count, void *cache, const int32_t *src, const int32_t *dst,
+                                                  void *stream);
+/* fork: row children[i] becomes what row parents[i] is.  Full pages are shared;
+ * a partly filled last page is copied to the lowest free page, handed out in the
+ * order of i and returned in fresh[i] (-1: none was needed).  fresh[i] = -2 and
+ * an empty row: no page was free, or the parent is no row.  No child is a parent,
+ * and a child's row holds no pages before. */
+int32_t baracuda_kernels_kv_pages_fork_gfx950_run(int32_t layers, int64_t num_pages, int64_t page_bytes,
+                                                  int32_t page_size, int32_t rows, int32_t max_pages, int32_t count,
+                                                  void *cache, int32_t *tables, int32_t *lens, int32_t *refs,
+                                                  const int32_t *parents, const int32_t *children, int32_t *fresh,
+                                                  void *stream);
+/* release: the rows which[i] give their pages back and are empty after. */
+int32_t baracuda_kernels_kv_pages_release_gfx950_run(int64_t num_pages, int32_t rows, int32_t max_pages, int32_t count,
+                                                     int32_t *tables, int32_t *lens, int32_t *refs,
+                                                     const int32_t *which, void *stream);
+/* compact: the pages in use, `live` of them, move to the front: the ones past the
+ * first `live`, lowest first, into the free ones before, lowest first.
+ * remap [num_pages]: the new place of a page, -1 for a free one; tables_out (may
+ * be tables) and refs_out (not refs) are the tables and counts after. */
+int32_t baracuda_kernels_kv_pages_compact_gfx950_run(
+    int32_t layers, int64_t num_pages, int64_t page_bytes, int32_t page_size, int32_t rows, int32_t max_pages, void *cache,
+    const int32_t *tables, const int32_t *refs, int32_t *tables_out, int32_t *refs_out, int32_t *remap, int32_t *live,
+    void *workspace, size_t workspace_bytes, void *stream);
+/* compact's workspace; required. */
+size_t baracuda_kernels_kv_pages_gfx950_workspace_size(int32_t layers, int64_t num_pages, int64_t page_bytes,
+                                                       int32_t page_size, int32_t rows, int32_t max_pages);
+int32_t baracuda_kernels_kv_pages_gfx950_can_implement(int32_t layers, int64_t num_pages, int64_t page_bytes,
+                                                       int32_t page_size, int32_t rows, int32_t max_pages);
 
 #ifdef __cplusplus
 }
