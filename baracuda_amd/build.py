@@ -23,10 +23,15 @@ LIB = PKG / "libbaracuda_kernels.so"
 # Measurement kernels of bench.py (not product), built beside the library.
 PROBES = PKG / "probes"
 PROBE_LIB = PKG / "libbaracuda_probes.so"
+# The plans' calls of the 4-bit cache's entry points, a Python module over torch's
+# headers (host code), beside the library that it calls.
+BINDING_SRC = CSRC / "kv4_binding.cpp"
+BINDING = PKG / "_kv4.so"
 # Digest of the sources and flags the library was built from, written beside it.
 STAMP = PKG / "libbaracuda_kernels.so.srchash"
 
 HIPCC = os.environ.get("HIPCC", shutil.which("hipcc") or "/opt/rocm/bin/hipcc")
+CXX = os.environ.get("CXX", "g++")
 ARCH = "gfx950"
 # -packed-fp32-ops: hipcc must not emit packed f32 VALU ops (v_pk_*_f32).
 # -ffp-contract=off: epilogue arithmetic is evaluated exactly as written, so
@@ -56,7 +61,7 @@ def source_digest() -> str:
     """SHA-256 over every kernel source, public header and the build flags."""
     h = hashlib.sha256()
     h.update(" ".join(HIP_FLAGS[:-2]).encode())
-    files = (sorted(CSRC.glob("*.hip")) + sorted(CSRC.glob("*.hpp")) + sorted((ROOT / "include").glob("*.h"))
+    files = (sorted(CSRC.glob("*.hip")) + sorted(CSRC.glob("*.hpp")) + sorted(CSRC.glob("*.cpp")) + sorted((ROOT / "include").glob("*.h"))
              + sorted(PROBES.glob("*.hip")))
     for f in files:
         h.update(f.name.encode())
@@ -66,7 +71,7 @@ def source_digest() -> str:
 
 def is_stale() -> bool:
     """True when the library is missing or was built from other sources."""
-    if not LIB.exists() or not STAMP.exists() or (any(PROBES.glob("*.hip")) and not PROBE_LIB.exists()):
+    if not LIB.exists() or not BINDING.exists() or not STAMP.exists() or (any(PROBES.glob("*.hip")) and not PROBE_LIB.exists()):
         return True
     return STAMP.read_text().strip() != source_digest()
 
@@ -92,12 +97,42 @@ def _build_probes() -> None:
     os.replace(tmp, PROBE_LIB)
 
 
+def _compile_binding() -> Path:
+    import sysconfig
+
+    import torch
+    from torch.utils.cpp_extension import include_paths
+
+    obj = BUILD / "kv4_binding.o"
+    dirs = [*include_paths(), sysconfig.get_paths()["include"], str(ROOT / "include")]
+    cmd = [CXX, "-O2", "-std=c++17", "-fPIC", "-fvisibility=hidden",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", *(f"-I{d}" for d in dirs),
+           "-c", str(BINDING_SRC), "-o", str(obj)]
+    res = subprocess.run(cmd, capture_output=True, text=True)
+    if res.returncode != 0:
+        raise RuntimeError(f"{CXX} failed for {BINDING_SRC.name}:\n{res.stderr}")
+    return obj
+
+
+def _link_binding(obj: Path) -> None:
+    import torch
+
+    tmp = BINDING.with_suffix(".so.tmp")
+    cmd = [CXX, "-shared", str(obj), f"-L{PKG}", "-l:libbaracuda_kernels.so", "-Wl,-rpath,$ORIGIN",
+           f"-L{Path(torch.__file__).parent / 'lib'}", "-ltorch_python", "-ltorch_cpu", "-lc10", "-o", str(tmp)]
+    res = subprocess.run(cmd, capture_output=True, text=True)
+    if res.returncode != 0:
+        raise RuntimeError(f"link failed for {BINDING.name}:\n{res.stderr}")
+    os.replace(tmp, BINDING)
+
+
 def build(verbose: bool = False) -> Path:
     """Compile every kernel source and link the shared library; returns its path."""
     BUILD.mkdir(exist_ok=True)
     digest = source_digest()
     sources = sorted(CSRC.glob("*.hip"))
     with cf.ThreadPoolExecutor(max_workers=min(8, len(sources))) as ex:
+        binding = ex.submit(_compile_binding)
         objs = list(ex.map(_compile, sources))
     tmp = LIB.with_suffix(".so.tmp")
     cmd = [HIPCC, f"--offload-arch={ARCH}", "-shared", "-fPIC", *map(str, objs), "-o", str(tmp)]
@@ -105,6 +140,7 @@ def build(verbose: bool = False) -> Path:
     if res.returncode != 0:
         raise RuntimeError(f"link failed:\n{res.stderr}")
     os.replace(tmp, LIB)
+    _link_binding(binding.result())
     _build_probes()
     STAMP.write_text(digest + "\n")
     if verbose:

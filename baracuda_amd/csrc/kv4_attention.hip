@@ -60,13 +60,14 @@ __device__ __forceinline__ int page_of(const AttnArgs &a, const int32_t *row, in
 }
 
 // MT tiles of 16 rows; NT tiles of 16 tokens a step; NW waves.
-template <typename T, int D, int MT, int NT, int NW>
-__global__ __launch_bounds__(64 * NW) void decode_kernel(const AttnArgs a) {
+template <typename T, int D, int MT, int NT, int NW, int OCC>
+__global__ __launch_bounds__(64 * NW, OCC) void decode_kernel(const AttnArgs a) {
     constexpr int RB = 16 * MT, KW = D / 32, OC = D / 16;
     constexpr int LD = D + 4;
     __shared__ float lds_m[NW][RB], lds_l[NW][RB];
     __shared__ __align__(16) float lds_o[NW][RB * LD];
     __shared__ Part lds_part;
+    __shared__ Item lds_item;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int r = lane & 15, g = lane >> 4;
     const int head = blockIdx.x % a.hk, index = blockIdx.x / a.hk;
@@ -74,15 +75,11 @@ __global__ __launch_bounds__(64 * NW) void decode_kernel(const AttnArgs a) {
     Part part;
     Item s;
     if (a.slots) {
-        if (wave == 0) {
-            part = find_part(a, RB, index);
-            if (lane == 0) lds_part = part;
-        }
+        if (wave == 0) find_part(a, RB, index, lds_part, lds_item);
         __syncthreads();
         part = lds_part;
-        part.item = __builtin_amdgcn_readfirstlane(part.item);
-        if (part.item < 0) return;
-        s = item_of(a, part.item, RB);
+        if (__builtin_amdgcn_readfirstlane(part.item) < 0) return;
+        s = lds_item;
     } else {
         s = item_of(a, index, RB);
         if (s.rows <= 0) return;
@@ -125,16 +122,29 @@ __global__ __launch_bounds__(64 * NW) void decode_kernel(const AttnArgs a) {
         for (int c = 0; c < OC; ++c) o[mt][c] = v4f{0, 0, 0, 0};
     }
 
-    for (int t = t0 + wave * NT; t < t1; t += NW * NT) {
-        Tile<D> tile[NT];
+    // the pages of this wave's next 64 / NT steps, a tile a lane
+    constexpr int kAhead = 64 / NT;
+    const auto pages_from = [&](int step) {
+        const int t = t0 + (step + lane / NT) * (NW * NT) + wave * NT + lane % NT;
+        return page_of(a, table, t, t1);
+    };
+    const int steps = max(0, (t1 - t0 - wave * NT + NW * NT - 1) / (NW * NT));
+    int pages = pages_from(0);
+    const auto load_step = [&](Tile<D> (&tile)[NT], int step) {
+        const int t = t0 + step * (NW * NT) + wave * NT;
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+            const int page = __builtin_amdgcn_readlane(pages, step % kAhead * NT + n);
+            load_tile<D>(tile[n], a, page < 0 ? 0 : page, head, (t + n) * 16 & (a.ps - 1), lane);
+        }
+    };
+    const auto do_step = [&](Tile<D> (&tile)[NT], int t, uint64_t held) {
         bool whole = 16 * t >= all_lo && 16 * (t + NT) <= all_hi && t + NT <= t1;
         bool there[NT];
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
-            const int page = page_of(a, table, t + n, t1);
-            there[n] = page >= 0;
+            there[n] = held >> n & 1;
             whole = whole && there[n];
-            load_tile<D>(tile[n], a, page < 0 ? 0 : page, head, (t + n) * 16 & (a.ps - 1), lane);
         }
         if (!whole) {
             // V of tokens that no row sees may be anything, also a NaN, and 0 times it would be one
@@ -162,7 +172,7 @@ __global__ __launch_bounds__(64 * NW) void decode_kernel(const AttnArgs a) {
             for (int mt = 0; mt < MT; ++mt) sc[mt][n] = v4f{0, 0, 0, 0};
 #pragma unroll
             for (int kk = 0; kk < KW; ++kk) {
-                const float ks = scale_value(D == 256 ? (tile[n].ks >> (kk >= 4 ? 8 : 0)) & 0xffu : tile[n].ks);
+                const float ks = scale_bits(D == 256 && kk < 4 ? tile[n].ks << 23 : D == 256 ? tile[n].ks << 15 : tile[n].ks << 23);
                 v4i f;
 #pragma unroll
                 for (int b = 0; b < 4; ++b) f[b] = (int)pair_of<T>(tile[n].k[kk], ks, b);
@@ -170,26 +180,23 @@ __global__ __launch_bounds__(64 * NW) void decode_kernel(const AttnArgs a) {
                 for (int mt = 0; mt < MT; ++mt) sc[mt][n] = mfma_pv<T>(f, q[mt][kk], sc[mt][n]);
             }
         }
-        // softmax
-        v4i p[MT][(NT + 1) / 2];
+        // softmax; m in units of the exponent
+        v4i p[MT][NT][2];
 #pragma unroll
         for (int mt = 0; mt < MT; ++mt) {
-            float top = m[mt];
+            float top = -INFINITY;
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
-                    float v = sc[mt][n][j] * a.scale;
                     if (!whole) {
                         const int tok = 16 * (t + n) + 4 * g + j;
-                        if (!there[n] || tok < lo[mt] || tok >= hi[mt]) v = -INFINITY;
+                        if (!there[n] || tok < lo[mt] || tok >= hi[mt]) sc[mt][n][j] = -INFINITY;
                     }
-                    sc[mt][n][j] = v;
-                    top = fmaxf(top, v);
+                    top = fmaxf(top, sc[mt][n][j]);
                 }
             }
-            top = fmaxf(top, __shfl_xor(top, 16, 64));
-            top = fmaxf(top, __shfl_xor(top, 32, 64));
+            top = fmaxf(max_over_groups(top) * a.scale, m[mt]);
             if (__any(top > m[mt])) {
                 const float f = top > m[mt] ? exp2_fast(m[mt] - top) : 1.0f;
                 l[mt] *= f;
@@ -197,53 +204,78 @@ __global__ __launch_bounds__(64 * NW) void decode_kernel(const AttnArgs a) {
                 for (int c = 0; c < OC; ++c) o[mt][c] *= f;
                 m[mt] = top;
             }
-            const float ref = m[mt] == -INFINITY ? 0.0f : m[mt];
+            const float ref = m[mt] == -INFINITY ? 0.0f : -m[mt];
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
                 float e[4];
 #pragma unroll
-                for (int j = 0; j < 4; ++j) e[j] = exp2_fast(sc[mt][n][j] - ref);
+                for (int j = 0; j < 4; ++j) {
+                    e[j] = exp2_fast(__builtin_fmaf(sc[mt][n][j], a.scale, ref));
+                    p[mt][n][0][j] = (int)pack2<T>(e[j], 0.0f);
+                    p[mt][n][1][j] = (int)pack2<T>(0.0f, e[j]);
+                }
                 l[mt] += (e[0] + e[1]) + (e[2] + e[3]);
-                p[mt][n / 2][(n & 1) * 2] = (int)pack2<T>(e[0], e[1]);
-                p[mt][n / 2][(n & 1) * 2 + 1] = (int)pack2<T>(e[2], e[3]);
             }
         }
-        // O^T += V^T P^T, two tiles of tokens a product
+        // O^T += V^T P^T.  A converted pair holds two values of one token, so the
+        // product runs over (token, value of the pair) with the weights of one of
+        // the two at a time: twice the matrix instructions, which have room, and
+        // none to bring tokens side by side.  The zeros meet values of the weighed
+        // ones' own group: where those are NaN, so are these.
 #pragma unroll
-        for (int n = 0; n < NT; n += 2) {
-            float vs[2][4];
-#pragma unroll
-            for (int h = 0; h < 2; ++h)
-#pragma unroll
-                for (int j = 0; j < 4; ++j) vs[h][j] = scale_value((tile[n + h].vs >> (8 * j)) & 0xffu);
+        for (int n = 0; n < NT; ++n) {
+            const float vs[4] = {scale_bits(tile[n].vs << 23), scale_bits(tile[n].vs << 15), scale_bits(tile[n].vs << 7),
+                                 scale_bits(tile[n].vs >> 1)};
 #pragma unroll
             for (int c = 0; c < D / 32; ++c) {
-                v4i even, odd;
+                v4i f;
 #pragma unroll
-                for (int h = 0; h < 2; ++h) {
-#pragma unroll
-                    for (int j = 0; j < 4; j += 2) {
-                        const int b0 = j * (D / 32) + c, b1 = (j + 1) * (D / 32) + c;
-                        const uint32_t x = pair_of<T>(tile[n + h].v[b0 / 4], vs[h][j], b0 % 4);
-                        const uint32_t y = pair_of<T>(tile[n + h].v[b1 / 4], vs[h][j + 1], b1 % 4);
-                        even[2 * h + j / 2] = (int)__builtin_amdgcn_perm(y, x, 0x05040100u);
-                        odd[2 * h + j / 2] = (int)__builtin_amdgcn_perm(y, x, 0x07060302u);
-                    }
+                for (int j = 0; j < 4; ++j) {
+                    const int b = j * (D / 32) + c;
+                    f[j] = (int)pair_of<T>(tile[n].v[b / 4], vs[j], b % 4);
                 }
 #pragma unroll
                 for (int mt = 0; mt < MT; ++mt) {
-                    o[mt][2 * c] = mfma_pv<T>(even, p[mt][n / 2], o[mt][2 * c]);
-                    o[mt][2 * c + 1] = mfma_pv<T>(odd, p[mt][n / 2], o[mt][2 * c + 1]);
+                    o[mt][2 * c] = mfma_pv<T>(f, p[mt][n][0], o[mt][2 * c]);
+                    o[mt][2 * c + 1] = mfma_pv<T>(f, p[mt][n][1], o[mt][2 * c + 1]);
                 }
             }
+        }
+    };
+    const auto held_of = [&](int step) { return __ballot(pages >= 0) >> (step % kAhead * NT) & ((1u << NT) - 1); };
+    if constexpr (NW >= 8) {
+        for (int i = 0; i < steps; ++i) {
+            if (i && i % kAhead == 0) pages = pages_from(i);
+            Tile<D> tile[NT];
+            load_step(tile, i);
+            do_step(tile, t0 + i * (NW * NT) + wave * NT, held_of(i));
+        }
+    } else if (steps) {
+        // the next step's loads go out before this one's products
+        Tile<D> even[NT], odd[NT];
+        load_step(even, 0);
+        uint64_t held = held_of(0);
+        for (int i = 0; i < steps; i += 2) {
+            uint64_t next = 0;
+            if (i + 1 < steps) {
+                load_step(odd, i + 1);
+                next = held_of(i + 1);
+            }
+            do_step(even, t0 + i * (NW * NT) + wave * NT, held);
+            if (i + 1 >= steps) break;
+            if (i + 2 < steps) {
+                if ((i + 2) % kAhead == 0) pages = pages_from(i + 2);
+                load_step(even, i + 2);
+                held = held_of(i + 2);
+            }
+            do_step(odd, t0 + (i + 1) * (NW * NT) + wave * NT, next);
         }
     }
 
     // join the waves: O relative to the workgroup's maximum of each row
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt) {
-        l[mt] += __shfl_xor(l[mt], 16, 64);
-        l[mt] += __shfl_xor(l[mt], 32, 64);
+        l[mt] = sum_over_groups(l[mt]);
         if (g == 0) lds_m[wave][16 * mt + r] = m[mt], lds_l[wave][16 * mt + r] = l[mt];
     }
     __syncthreads();
@@ -294,50 +326,95 @@ __global__ __launch_bounds__(64 * NW) void decode_kernel(const AttnArgs a) {
     }
 }
 
-// Joins the parts of the rows of items that were cut.  A wave a row.
-template <typename T, int D, int RB>
+// Joins the parts of the rows of items that were cut: W waves a row take the
+// parts in turn, eight parts' values in flight in each.  With few rows there are
+// waves to spare: two sequences of 64 heads and 32 parts take 4.7 us with four
+// waves a row and 8.0 with one, 24 sequences of 200 rows 6.7 and 4.0.
+template <typename T, int D, int RB, int W>
 __global__ __launch_bounds__(256) void join_kernel(const AttnArgs a, int64_t all) {
-    constexpr int V = D / 64;
-    const int lane = threadIdx.x & 63;
-    const int item = blockIdx.x / a.hk, head = blockIdx.x % a.hk;
-    const int row = __builtin_amdgcn_readfirstlane(blockIdx.y * 4 + (threadIdx.x >> 6));
-    const Item s = item_of(a, item, RB);
-    if (row >= s.rows) return;
+    constexpr int V = D / 64, U = 8;
+    typedef float vec __attribute__((ext_vector_type(V)));
+    __shared__ float lds_m[W], lds_l[W];
+    __shared__ vec lds_o[W][64];
+    const int lane = threadIdx.x & 63, id = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int wave = W == 1 ? 0 : id;
+    const int item = blockIdx.x / a.hk, head = blockIdx.x % a.hk, row = W == 1 ? blockIdx.y * 4 + id : blockIdx.y;
     const int2 cut = ((const int2 *)a.split)[item];
-    if (cut.y < 2) return;
+    const Item s = item_of(a, item, RB);
+    if (row >= s.rows || cut.y < 2) return;
     const float *ml = (const float *)(a.split + a.part);
     const float *o = ml + 2 * all + lane * V;
-    float top = -INFINITY;
-    for (int k = lane; k < cut.y; k += 64) top = fmaxf(top, ml[2 * (((int64_t)(cut.x + k) * a.hk + head) * RB + row)]);
+    const auto place = [&](int k) { return ((int64_t)(cut.x + k) * a.hk + head) * RB + row; };
+    float top = -INFINITY, sum = 0.0f;
+    vec acc = 0.0f;
+    for (int k0 = wave; k0 < cut.y; k0 += W * U) {
+        float m[U], l[U];
+        vec x[U];
 #pragma unroll
-    for (int x = 1; x < 64; x *= 2) top = fmaxf(top, __shfl_xor(top, x, 64));
-    float sum = 0.0f, acc[V];
+        for (int u = 0; u < U; ++u) {
+            const int64_t at = place(min(k0 + W * u, cut.y - 1));
+            m[u] = ml[2 * at], l[u] = ml[2 * at + 1];
+            x[u] = *(const vec *)(o + at * D);
+        }
+        float high = top;
 #pragma unroll
-    for (int v = 0; v < V; ++v) acc[v] = 0.0f;
-    for (int k = 0; k < cut.y; ++k) {
-        const int64_t at = ((int64_t)(cut.x + k) * a.hk + head) * RB + row;
-        const float mk = ml[2 * at], lk = ml[2 * at + 1];
-        const float f = mk == -INFINITY ? 0.0f : exp2_fast(mk - top);
-        sum += lk == lk ? lk * f : lk;
+        for (int u = 0; u < U; ++u) {
+            if (k0 + W * u >= cut.y) m[u] = -INFINITY, l[u] = 0.0f, x[u] = 0.0f;
+            high = fmaxf(high, m[u]);
+        }
+        const float f = top == -INFINITY ? 0.0f : exp2_fast(top - high);
+        sum *= f;
+        acc *= f;
+        top = high;
 #pragma unroll
-        for (int v = 0; v < V; ++v) acc[v] += o[at * D + v] * f;
+        for (int u = 0; u < U; ++u) {
+            const float e = m[u] == -INFINITY ? (l[u] == l[u] ? 0.0f : l[u]) : exp2_fast(m[u] - top);
+            sum += l[u] * e;
+            acc += x[u] * e;
+        }
+    }
+    if constexpr (W > 1) {
+        lds_o[wave][lane] = acc;
+        if (lane == 0) lds_m[wave] = top, lds_l[wave] = sum;
+        __syncthreads();
+        if (wave) return;
+#pragma unroll
+        for (int w = 0; w < W; ++w) top = fmaxf(top, lds_m[w]);
+        sum = 0.0f;
+        acc = 0.0f;
+#pragma unroll
+        for (int w = 0; w < W; ++w) {
+            const float mw = lds_m[w], lw = lds_l[w];
+            const float e = mw == -INFINITY ? (lw == lw ? 0.0f : lw) : exp2_fast(mw - top);
+            sum += lw * e;
+            acc += lds_o[w][lane] * e;
+        }
     }
     const float inv = sum > 0.0f || sum != sum ? 1.0f / sum : 0.0f;
     const int x = s.first + row;
     uint16_t *dst = (uint16_t *)a.out + (s.q0 + x / a.ratio) * a.out_token + (head * a.ratio + x % a.ratio) * a.out_head + lane * V;
+    if constexpr (V == 1) {
+        dst[0] = (uint16_t)pack2<T>(acc[0] * inv, 0.0f);
+    } else {
+        typedef struct __attribute__((packed, aligned(2))) { uint32_t w[V / 2]; } Out;
+        Out out;
 #pragma unroll
-    for (int v = 0; v < V; ++v) dst[v] = (uint16_t)pack2<T>(acc[v] * inv, 0.0f);
+        for (int v = 0; v < V; v += 2) out.w[v / 2] = pack2<T>(acc[v] * inv, acc[v + 1] * inv);
+        *(Out *)dst = out;
+    }
 }
 
 // How a problem is cut, the same for the workspace's size and the launch.
 struct Cut {
     int mt, rows, row_blocks, slots, min_tiles;
+    bool wide;                // one workgroup of many waves has a whole sequence
     int64_t items, grid;
     size_t part, bytes;
 };
 
 constexpr int kSlots = 512;
 constexpr int kMinTiles = 16;
+constexpr int kJoinWide = 2048;   // rows up to which four waves join one
 constexpr int kWhole = 1024;      // tokens up to which nothing is cut
 
 Cut cut_of(int num_seqs, int max_q, int64_t max_kv, int ratio, int hk, int D, int window) {
@@ -349,6 +426,7 @@ Cut cut_of(int num_seqs, int max_q, int64_t max_kv, int ratio, int hk, int D, in
     const int64_t seen = window && window + (int64_t)max_q < max_kv ? window + (int64_t)max_q : max_kv;
     c.slots = seen <= kWhole || c.items * hk >= 8 * kSlots ? 0 : kSlots;
     c.min_tiles = kMinTiles;
+    c.wide = !c.slots && c.mt == 1 && seen > 256 && c.items * hk <= 256;
     c.grid = c.items * hk + c.slots;
     if (c.slots) {
         c.grid = (c.grid + hk - 1) / hk * hk;
@@ -360,15 +438,26 @@ Cut cut_of(int num_seqs, int max_q, int64_t max_kv, int ratio, int hk, int D, in
 
 template <typename T, int D>
 int32_t launch_attention(AttnArgs a, const Cut &c, hipStream_t stream) {
-    constexpr int NT = D == 256 ? 2 : 4;
+    constexpr int WIDE = D == 256 ? 8 : 16, TWO = D == 256 ? 2 : 4;
     const dim3 grid((unsigned)c.grid);
-    if (c.mt == 1) hipLaunchKernelGGL((decode_kernel<T, D, 1, NT, 4>), grid, dim3(256), 0, stream, a);
-    else hipLaunchKernelGGL((decode_kernel<T, D, 2, NT, D == 256 ? 2 : 4>), grid, dim3(D == 256 ? 128 : 256), 0, stream, a);
+    if (c.mt == 2)
+        hipLaunchKernelGGL((decode_kernel<T, D, 2, 2, TWO, 2>), grid, dim3(64 * TWO), 0, stream, a);
+    else if (c.wide)
+        hipLaunchKernelGGL((decode_kernel<T, D, 1, 2, WIDE, WIDE / 4>), grid, dim3(64 * WIDE), 0, stream, a);
+    else
+        hipLaunchKernelGGL((decode_kernel<T, D, 1, 2, 4, D == 256 ? 2 : 3>), grid, dim3(256), 0, stream, a);
     const int32_t st = launch_status();
     if (st != kOk || !c.slots) return st;
-    const dim3 rows((unsigned)(c.items * a.hk), (unsigned)((c.rows + 3) / 4));
-    if (c.mt == 1) hipLaunchKernelGGL((join_kernel<T, D, 16>), rows, dim3(256), 0, stream, a, c.grid * 16);
-    else hipLaunchKernelGGL((join_kernel<T, D, 32>), rows, dim3(256), 0, stream, a, c.grid * 32);
+    const int items = (int)c.items * a.hk;
+    if (items * c.rows <= kJoinWide) {
+        const dim3 grid((unsigned)items, (unsigned)c.rows);
+        if (c.mt == 1) hipLaunchKernelGGL((join_kernel<T, D, 16, 4>), grid, dim3(256), 0, stream, a, c.grid * 16);
+        else hipLaunchKernelGGL((join_kernel<T, D, 32, 4>), grid, dim3(256), 0, stream, a, c.grid * 32);
+    } else {
+        const dim3 grid((unsigned)items, (unsigned)((c.rows + 3) / 4));
+        if (c.mt == 1) hipLaunchKernelGGL((join_kernel<T, D, 16, 1>), grid, dim3(256), 0, stream, a, c.grid * 16);
+        else hipLaunchKernelGGL((join_kernel<T, D, 32, 1>), grid, dim3(256), 0, stream, a, c.grid * 32);
+    }
     return launch_status();
 }
 

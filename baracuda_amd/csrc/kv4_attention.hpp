@@ -71,10 +71,36 @@ __device__ __forceinline__ void row_span(const AttnArgs &a, const Item &s, int r
     lo = in && a.window ? max(0, pos - a.window + 1) : 0;
 }
 
-__device__ __forceinline__ int wave_sum(int x) {
+__device__ __forceinline__ float as_float(uint32_t x) { return __uint_as_float(x); }
+
+// Lanes that differ in bit 4, and in bit 5: the four groups of 16 that hold
+// the same row (v_permlane*_swap: no trip through LDS).
+__device__ __forceinline__ float max_over_groups(float x) {
+    const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    x = fmaxf(as_float(a[0]), as_float(a[1]));
+    const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return fmaxf(as_float(b[0]), as_float(b[1]));
+}
+__device__ __forceinline__ float sum_over_groups(float x) {
+    const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    x = as_float(a[0]) + as_float(a[1]);
+    const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return as_float(b[0]) + as_float(b[1]);
+}
+
+template <typename X>
+__device__ __forceinline__ X wave_sum(X x) {
 #pragma unroll
     for (int m = 1; m < 64; m *= 2) x += __shfl_xor(x, m, 64);
     return x;
+}
+__device__ __forceinline__ float wave_max(float x) {
+#pragma unroll
+    for (int m = 1; m < 64; m *= 2) x = fmaxf(x, __shfl_xor(x, m, 64));
+    return x;
+}
+__device__ __forceinline__ float lane_value(float x, int lane) {
+    return __uint_as_float((uint32_t)__builtin_amdgcn_readlane((int)__float_as_uint(x), lane));
 }
 
 // A part of an item: tiles [t0, t1) of 16 tokens.  `parts` parts have the item,
@@ -83,29 +109,29 @@ struct Part {
     int item, t0, t1, parts, begin;
 };
 
-// Part `index` of all, worked out from the lengths by one wave: all items
-// together are cut into about slots / hk parts of one size, so that the
-// longest sequence does not hold up the launch.  Items of one wave's width
-// cost one pass over the lengths.  item < 0: there is no such part.
-__device__ __forceinline__ Part find_part(const AttnArgs &a, int block, int index) {
+// Part `index` of all, and its item, worked out from the lengths by one wave: all
+// items together are cut into about slots / hk parts of one size, so that the
+// longest sequence does not hold up the launch.  Up to 64 items cost one pass
+// over the lengths.  part.item < 0: there is no such part.
+__device__ __forceinline__ void find_part(const AttnArgs &a, int block, int index, Part &part, Item &item) {
     const int lane = threadIdx.x & 63;
+    Item s;
     int total = 0;
     for (int i0 = 0; i0 < a.items; i0 += 64) {
-        const int i = i0 + lane;
-        total += wave_sum(i < a.items ? tiles_of(item_of(a, i, block)) : 0);
+        s.rows = s.lo = s.hi = 0;
+        if (i0 + lane < a.items) s = item_of(a, i0 + lane, block);
+        total += tiles_of(s);
     }
+    total = wave_sum(total);
     const int per = max(a.min_tiles, (int)(((int64_t)total * a.hk + a.slots - 1) / a.slots));
-    Part p{-1, 0, 0, 0, 0};
     int begin = 0;
     for (int i0 = 0; i0 < a.items; i0 += 64) {
-        const int i = i0 + lane;
-        int n = 0, tiles = 0, lo = 0;
-        if (i < a.items) {
-            const Item s = item_of(a, i, block);
-            tiles = tiles_of(s);
-            lo = s.lo / 16;
-            n = s.rows > 0 ? max(1, (tiles + per - 1) / per) : 0;
+        if (a.items > 64) {
+            s.rows = s.lo = s.hi = 0;
+            if (i0 + lane < a.items) s = item_of(a, i0 + lane, block);
         }
+        const int tiles = tiles_of(s);
+        const int n = s.rows > 0 ? max(1, (tiles + per - 1) / per) : 0;
         int sum = n;
 #pragma unroll
         for (int d = 1; d < 64; d *= 2) {
@@ -113,23 +139,17 @@ __device__ __forceinline__ Part find_part(const AttnArgs &a, int block, int inde
             if (lane >= d) sum += o;
         }
         const int mine = begin + sum - n;
-        const uint64_t hit = __ballot(index >= mine && index < mine + n);
+        const bool hit = index >= mine && index < mine + n;
         if (hit) {
-            const int src = __builtin_ctzll(hit);
-            p.item = i0 + src;
-            p.parts = __shfl(n, src, 64);
-            p.begin = __shfl(mine, src, 64);
-            tiles = __shfl(tiles, src, 64);
-            lo = __shfl(lo, src, 64);
             // equal parts of the item
-            const int each = (tiles + p.parts - 1) / p.parts, k = index - p.begin;
-            p.t0 = lo + min(tiles, k * each);
-            p.t1 = lo + min(tiles, (k + 1) * each);
-            return p;
+            const int each = (tiles + n - 1) / n, k = index - mine, t0 = s.lo / 16;
+            part = Part{i0 + lane, t0 + min(tiles, k * each), t0 + min(tiles, (k + 1) * each), n, mine};
+            item = s;
         }
+        if (__any(hit)) return;
         begin += __shfl(sum, 63, 64);
     }
-    return p;
+    if (lane == 0) part.item = -1;
 }
 
 template <typename T>
@@ -174,6 +194,10 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
         return (uint32_t)f32_to_f16_rne(lo) | (uint32_t)f32_to_f16_rne(hi) << 16;
     }
 }
+
+// The scale of a conversion: the instruction reads the exponent alone, and 255
+// there makes its results NaN, so the bits around the byte may be anything.
+__device__ __forceinline__ float scale_bits(uint32_t x) { return __uint_as_float(x); }
 
 __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
 

@@ -52,50 +52,81 @@ __device__ __forceinline__ float inv_root<float>(float x) { return 1.0f / __buil
 template <>
 __device__ __forceinline__ double inv_root<double>(double x) { return 1.0 / __builtin_sqrt(x); }
 
-// The norm and the rotation of one head, eight values a lane, in type A.
-template <typename A, int G, bool INTER>
-__device__ __forceinline__ void norm_rope(const float (&x)[8], float (&y)[8], const float (&w)[8], bool norm, double eps,
-                                          int D, bool turn, int partner, const float (&c)[8], const float (&s)[8]) {
-    A v[8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = (A)x[i];
+// Lane exchanges within the G lanes of a head, for a sum: after step k all
+// lanes of 2^(k+1) hold the same, so a mirrored lane serves as well as the one
+// across.  DPP and v_permlane16_swap: no trip through LDS.
+template <int M>
+__device__ __forceinline__ uint32_t across(uint32_t x) {
+    constexpr int ctrl = M == 1 ? 0xB1 : M == 2 ? 0x4E : M == 4 ? 0x141 : 0x140;
+    return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, ctrl, 0xf, 0xf, true);
+}
+template <int M>
+__device__ __forceinline__ float add_across(float x) {
+    if constexpr (M == 16) {
+        const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+        return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+    } else {
+        return x + __uint_as_float(across<M>(__float_as_uint(x)));
+    }
+}
+template <int M>
+__device__ __forceinline__ double add_across(double x) {
+    const uint64_t b = __builtin_bit_cast(uint64_t, x);
+    if constexpr (M == 16) {
+        const auto lo = __builtin_amdgcn_permlane16_swap((uint32_t)b, (uint32_t)b, false, false);
+        const auto hi = __builtin_amdgcn_permlane16_swap((uint32_t)(b >> 32), (uint32_t)(b >> 32), false, false);
+        return __builtin_bit_cast(double, (uint64_t)hi[0] << 32 | lo[0]) +
+               __builtin_bit_cast(double, (uint64_t)hi[1] << 32 | lo[1]);
+    } else {
+        const uint64_t o = (uint64_t)across<M>((uint32_t)(b >> 32)) << 32 | across<M>((uint32_t)b);
+        return x + __builtin_bit_cast(double, o);
+    }
+}
+template <typename A, int G>
+__device__ __forceinline__ A head_sum(A x) {
+    x = add_across<1>(x);
+    x = add_across<2>(x);
+    x = add_across<4>(x);
+    if constexpr (G >= 16) x = add_across<8>(x);
+    if constexpr (G >= 32) x = add_across<16>(x);
+    return x;
+}
+
+// The norm and the rotation of one head in type A: eight values a lane (x), the
+// other sides of their pairs (z) and both sides' weights.
+template <typename A, int G>
+__device__ __forceinline__ void norm_rope(const float (&x)[8], const float (&z)[8], float (&y)[8], const float (&w)[8],
+                                          const float (&wz)[8], bool norm, double eps, int D, bool turn, const float (&c)[8],
+                                          const float (&s)[8]) {
+    A r = 1;
     if (norm) {
         A sum = 0;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) sum = __builtin_elementwise_fma(v[i], v[i], sum);
-#pragma unroll
-        for (int m = 1; m < G; m *= 2) sum += __shfl_xor(sum, m, G);
-        const A r = inv_root<A>(sum / (A)D + (A)eps);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = v[i] * r * (A)w[i];
-    }
-    A o[8];
-    if constexpr (INTER) {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) o[i] = v[i ^ 1];
-    } else {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) o[i] = __shfl(v[i], partner, G);
+        for (int i = 0; i < 8; ++i) sum = __builtin_elementwise_fma((A)x[i], (A)x[i], sum);
+        r = inv_root<A>(head_sum<A, G>(sum) / (A)D + (A)eps);
     }
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-        const A t = __builtin_elementwise_fma(v[i], (A)c[i], o[i] * (A)s[i]);
-        y[i] = (float)(turn ? t : v[i]);
+        A v = (A)x[i], o = (A)z[i];
+        if (norm) v = v * r * (A)w[i], o = o * r * (A)wz[i];
+        const A t = __builtin_elementwise_fma(v, (A)c[i], o * (A)s[i]);
+        y[i] = (float)(turn ? t : v);
     }
 }
 
-// G lanes a head, ITERS heads a lane.  T: the element; KV4: K and V go into the cache.
-template <typename T, int G, int ITERS, bool INTER, bool KV4>
-__global__ __launch_bounds__(64 * kWaves) void rows_kernel(const RowArgs a) {
+// G lanes a head, ITERS heads a lane, `share` of the workgroup's waves a token.
+// T: the element; KV4: K and V go into the cache.
+template <typename T, int G, int ITERS, bool KV4>
+__global__ __launch_bounds__(64 * kWaves) void rows_kernel(const RowArgs a, int share, bool inter) {
     typedef typename Raw<T>::Mem Mem;
-    constexpr int HPW = 64 / G;
-    const int64_t token = blockIdx.x;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    constexpr int HPW = 64 / G, W = sizeof(Mem) / 4;
+    __shared__ __align__(16) float lds_c[kWaves][128], lds_s[kWaves][128];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int64_t token = (int64_t)blockIdx.x * (kWaves / share) + wave / share;
     const int l = lane % G, at = 8 * l;
     const int heads = a.hq + a.hk * (KV4 ? 2 : 1);
-    const int first = (blockIdx.y * kWaves + wave) * HPW * ITERS + lane / G;
-    if (first - lane / G >= heads) return;
-    const bool mine = at < a.D;
+    const int first = (blockIdx.y * share + wave % share) * HPW * ITERS + lane / G;
+    const bool here = token < a.tokens, mine = here && at < a.D;
 
     Mem raw[ITERS];
 #pragma unroll
@@ -110,53 +141,75 @@ __global__ __launch_bounds__(64 * kWaves) void rows_kernel(const RowArgs a) {
         }
     }
 
-    // this lane's cosines and sines, the sine with the sign of its side
-    float c[8], s[8];
-    const bool turn = at < a.rope;
+    // the token's cosines and sines, once for all its heads, through LDS
     const int half = a.rope / 2;
-    const int partner = INTER ? l : turn ? (at < half ? l + half / 8 : l - half / 8) : l;
-    if (turn) {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const int pair = INTER ? (at + i) / 2 : at < half ? at + i : at + i - half;
-            const int axis = a.pair_axis ? a.pair_axis[pair] : 0;
+    float *lc = lds_c[wave / share], *ls = lds_s[wave / share];
+    if (here) {
+        for (int p = wave % share * 64 + lane; p < half; p += 64 * share) {
+            const int axis = a.pair_axis ? a.pair_axis[p] : 0;
             int64_t row = -1;
             if ((unsigned)axis < (unsigned)a.axes) row = a.positions[(int64_t)axis * a.tokens + token];
             const bool ok = row >= 0 && row < a.table_rows;
-            const int64_t e = row * half + pair;
-            c[i] = ok ? a.cosine[e] : __uint_as_float(0x7fc00000u);
-            const float sn = ok ? a.sine[e] : 0.0f;
-            const bool low = INTER ? (i & 1) == 0 : at < half;
-            s[i] = low ? -sn : sn;
+            lc[p] = ok ? a.cosine[row * half + p] : __uint_as_float(0x7fc00000u);
+            ls[p] = ok ? a.sine[row * half + p] : 0.0f;
         }
     }
 
+    // this lane's, the sine with the sign of its side, and the lane that holds
+    // the other side of its pairs (its own when interleaved)
+    const bool turn = at < a.rope, low = at < half;
+    const int other = inter || !turn ? l : low ? l + half / 8 : l - half / 8;
     const bool norm = a.weight[0] != nullptr;
-    float wq[8], wk[8];
+    float w[2][8], wz[2][8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) wq[i] = wk[i] = 0.0f;
-    if (norm && mine) {
-        const Mem mq = *(const Mem *)((const char *)a.weight[0] + (int64_t)at * (sizeof(Mem) / 8));
-        const Mem mk = *(const Mem *)((const char *)a.weight[1] + (int64_t)at * (sizeof(Mem) / 8));
+    for (int k = 0; k < 2; ++k) {
+        Mem m{}, z{};
+        if (norm && at < a.D) {
+            m = *(const Mem *)((const char *)a.weight[k] + (int64_t)at * (sizeof(Mem) / 8));
+            z = *(const Mem *)((const char *)a.weight[k] + (int64_t)(8 * other) * (sizeof(Mem) / 8));
+        }
 #pragma unroll
-        for (int i = 0; i < 8; ++i) wq[i] = Raw<T>::get(mq, i), wk[i] = Raw<T>::get(mk, i);
+        for (int i = 0; i < 8; ++i) w[k][i] = Raw<T>::get(m, i), wz[k][i] = Raw<T>::get(z, inter ? i ^ 1 : i);
+    }
+    int64_t slot = 0;
+    if constexpr (KV4) slot = here ? a.slots[token] : -1;
+    __syncthreads();
+    if (!here) return;
+    float c[8], s[8];
+    if (turn) {
+        const int p0 = inter ? at / 2 : low ? at : at - half;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const int p = p0 + (inter ? i / 2 : i);
+            c[i] = lc[p];
+            s[i] = (inter ? (i & 1) == 0 : low) ? -ls[p] : ls[p];
+        }
     }
 
-    int64_t slot = 0;
-    if constexpr (KV4) slot = a.slots[token];
 #pragma unroll
     for (int it = 0; it < ITERS; ++it) {
         const int h = first + it * HPW;
+        if (h - lane / G >= heads) break;
         const int kind = h < a.hq ? 0 : h < a.hq + a.hk ? 1 : 2;
         const int hh = h - (kind == 0 ? 0 : kind == 1 ? a.hq : a.hq + a.hk);
-        float x[8], y[8];
+        float x[8], z[8], y[8];
 #pragma unroll
         for (int i = 0; i < 8; ++i) x[i] = Raw<T>::get(raw[it], i);
-        if (!KV4 || kind == 0) {
-            float w[8];
+        if (inter) {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) w[i] = kind ? wk[i] : wq[i];
-            norm_rope<float, G, INTER>(x, y, w, norm, a.eps, a.D, turn, partner, c, s);
+            for (int i = 0; i < 8; ++i) z[i] = x[i ^ 1];
+        } else {
+            Mem m;
+#pragma unroll
+            for (int i = 0; i < W; ++i) m.w[i] = (uint32_t)__shfl((int)raw[it].w[i], other, G);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) z[i] = Raw<T>::get(m, i);
+        }
+        if (!KV4 || kind == 0) {
+            float wh[8], wo[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) wh[i] = w[KV4 ? 0 : kind == 1][i], wo[i] = wz[KV4 ? 0 : kind == 1][i];
+            norm_rope<float, G>(x, z, y, wh, wo, norm, a.eps, a.D, turn, c, s);
             if (mine && h < heads) {
                 Mem out;
                 Raw<T>::put(out, y);
@@ -165,7 +218,7 @@ __global__ __launch_bounds__(64 * kWaves) void rows_kernel(const RowArgs a) {
             }
         } else if constexpr (KV4) {
             if (kind == 1) {
-                norm_rope<double, G, INTER>(x, y, wk, norm, a.eps, a.D, turn, partner, c, s);
+                norm_rope<double, G>(x, z, y, w[1], wz[1], norm, a.eps, a.D, turn, c, s);
 #pragma unroll
                 for (int i = 0; i < 8; ++i) y[i] = Raw<T>::round(y[i]);
             } else {
@@ -176,8 +229,8 @@ __global__ __launch_bounds__(64 * kWaves) void rows_kernel(const RowArgs a) {
             uint32_t top = 0;
 #pragma unroll
             for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(y[i]) & 0x7fffffffu);
-            top = max(top, (uint32_t)__shfl_xor((int)top, 1, G));
-            top = max(top, (uint32_t)__shfl_xor((int)top, 2, G));
+            top = max(top, across<1>(top));
+            top = max(top, across<2>(top));
             const bool good = top < 0x7f800000u;
             const int byte = good ? scale_byte(top, a.most) : 255;
             const uint32_t code = good ? encode8(y, byte) : 0u;
@@ -247,30 +300,24 @@ __global__ __launch_bounds__(256) void read_kernel(const uint8_t *__restrict__ c
     }
 }
 
-template <typename T, int G, int ITERS, bool INTER, bool KV4>
-void launch_rows(const RowArgs &a, hipStream_t stream) {
-    const int heads = a.hq + a.hk * (KV4 ? 2 : 1);
-    const int per = (64 / G) * ITERS * kWaves;
-    hipLaunchKernelGGL((rows_kernel<T, G, ITERS, INTER, KV4>), dim3((unsigned)a.tokens, (unsigned)((heads + per - 1) / per)),
-                       dim3(64 * kWaves), 0, stream, a);
-}
-
-template <typename T, int G, bool INTER, bool KV4>
-void launch_iters(const RowArgs &a, hipStream_t stream) {
-    launch_rows<T, G, 1, INTER, KV4>(a, stream);
-}
-
-template <typename T, bool INTER, bool KV4>
-void launch_lanes(const RowArgs &a, hipStream_t stream) {
-    if (a.D <= 64) launch_iters<T, 8, INTER, KV4>(a, stream);
-    else if (a.D <= 128) launch_iters<T, 16, INTER, KV4>(a, stream);
-    else launch_iters<T, 32, INTER, KV4>(a, stream);
+template <typename T, int G, bool KV4>
+void launch_lanes(const RowArgs &a, bool inter, hipStream_t stream) {
+    const int heads = a.hq + a.hk * (KV4 ? 2 : 1), rounds = (heads + 64 / G - 1) / (64 / G);
+    // a wave has up to three rounds of heads of a token where there are tokens
+    // enough to fill the card without cutting them finer
+    const int iters = rounds > 2 * kWaves && a.tokens >= 512 ? 3 : 1;
+    const int waves = (rounds + iters - 1) / iters;
+    const int share = waves >= 3 ? 4 : waves;
+    const dim3 grid((unsigned)((a.tokens + kWaves / share - 1) / (kWaves / share)), (unsigned)((waves + share - 1) / share));
+    if (iters == 3) hipLaunchKernelGGL((rows_kernel<T, G, 3, KV4>), grid, dim3(64 * kWaves), 0, stream, a, share, inter);
+    else hipLaunchKernelGGL((rows_kernel<T, G, 1, KV4>), grid, dim3(64 * kWaves), 0, stream, a, share, inter);
 }
 
 template <typename T, bool KV4>
-int32_t launch_style(const RowArgs &a, bool interleaved, hipStream_t stream) {
-    if (interleaved) launch_lanes<T, true, KV4>(a, stream);
-    else launch_lanes<T, false, KV4>(a, stream);
+int32_t launch_style(const RowArgs &a, bool inter, hipStream_t stream) {
+    if (a.D <= 64) launch_lanes<T, 8, KV4>(a, inter, stream);
+    else if (a.D <= 128) launch_lanes<T, 16, KV4>(a, inter, stream);
+    else launch_lanes<T, 32, KV4>(a, inter, stream);
     return launch_status();
 }
 

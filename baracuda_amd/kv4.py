@@ -9,7 +9,8 @@
 No counterpart in the reference.  The manner is that of ``plans``: ``select`` a
 plan for a descriptor, ``run`` it on a stream (torch's current one by default);
 ``run`` neither allocates nor synchronises, so it can be captured into a graph,
-and errors are the exceptions of ``plans``.
+and errors are the exceptions of ``plans``.  Operands are checked
+against the descriptor in the binding (csrc/kv4_binding.cpp), before any launch.
 
 The cache is a uint8 tensor [pages, kv heads, kv4.head_bytes(page size, D)], two
 codes a byte (sign, two exponent bits, one mantissa bit); 32 values share a
@@ -17,16 +18,30 @@ power of two.  include/baracuda_kernels.h describes its bytes.
 """
 from __future__ import annotations
 
+import struct
 from dataclasses import dataclass
 from typing import Optional
 
 import torch
 
 from .ffi import lib
-from .plans import ElementKind, InvalidProblem, Unsupported, _nbytes, _need, _ptr, _stream, check
+from .plans import ElementKind, InvalidProblem, Unsupported, _need, check
+
+try:
+    from . import _kv4
+except ImportError as e:      # no fallback: the operands' checks and the calls are in it
+    raise RuntimeError("baracuda_amd/_kv4.so is missing or does not fit: build it with "
+                       "`python -m baracuda_amd.build`") from e
+
+
+def _raw_stream(device: int) -> int:
+    return torch.cuda.current_stream(device).cuda_stream
+
+
+# torch's own lookup by device index where it has one: no Stream object for each call
+_kv4.connect(InvalidProblem, getattr(torch._C, "_cuda_getCurrentRawStream", _raw_stream))
 
 _TAG = {ElementKind.F32: 0, ElementKind.F16: 1, ElementKind.Bf16: 2}
-_DTYPE = {ElementKind.F32: torch.float32, ElementKind.F16: torch.float16, ElementKind.Bf16: torch.bfloat16}
 
 
 def head_bytes(page_size: int, head_dim: int) -> int:
@@ -40,62 +55,21 @@ def _element(desc) -> int:
     return _TAG[desc.element]
 
 
-def _heads(t: Optional[torch.Tensor], tokens: int, heads: int, dim: int, dtype, what: str) -> None:
-    _need(t is not None, f"{what} is required")
-    _need(tuple(t.shape) == (tokens, heads, dim) and t.dtype == dtype,
-          f"{what} must be {dtype} [{tokens}, {heads}, {dim}]")
-    _need(dim <= 1 or t.stride(2) == 1, f"{what}: the values of a head must be dense")
+_INT64 = ("tokens", "num_pages", "max_kv", "page_bytes")
 
 
-def _out(t: torch.Tensor, what: str) -> None:
-    """An output whose elements are all in places of their own."""
-    t0, t1, dim = t.stride(0), t.stride(1), t.shape[2]
-    dense = (t.shape[1] <= 1 or t1 >= dim) and (t.shape[0] <= 1 or t0 >= (t.shape[1] - 1) * t1 + dim)
-    heads_first = t.shape[0] <= 1 or (t0 >= dim and (t.shape[1] <= 1 or t1 >= (t.shape[0] - 1) * t0 + dim))
-    _need(t.numel() == 0 or dense or heads_first, f"{what}: rows must not overlap")
+def _sizes_fit(desc) -> None:
+    """Sizes as the C entries take them: 64 bits for the long ones, 32 for the others."""
+    for name, value in vars(desc).items():
+        if isinstance(value, int) and not -2 ** 31 <= value < 2 ** (63 if name in _INT64 else 31):
+            raise Unsupported(f"{name} = {value}")
 
 
-def _ints(t: Optional[torch.Tensor], shape: tuple, what: str, dtype=torch.int32) -> None:
-    _need(t is not None, f"{what} is required")
-    _need(tuple(t.shape) == shape and t.dtype == dtype and t.is_contiguous(),
-          f"{what} must be contiguous {dtype} {list(shape)}")
-
-
-def _row(t: torch.Tensor) -> tuple:
-    return t.stride(0), t.stride(1)
-
-
-def _one_device(*tensors) -> None:
-    """All operands on one GPU; the launch goes to that GPU's stream."""
-    found = {t.device for t in tensors if t is not None and t.is_cuda}
-    _need(len(found) <= 1, "operands must be on one GPU")
-
-
-def _rotation(d, q_weight, k_weight, positions, cos, sin, pair_axis) -> list:
-    """Checks and C arguments of the norms' weights and the rotation's table."""
-    dtype = _DTYPE[d.element]
-    if d.norm:
-        for w, what in ((q_weight, "q_weight"), (k_weight, "k_weight")):
-            _ints(w, (d.head_dim,), what, dtype)
-    else:
-        _need(q_weight is None and k_weight is None, "a descriptor without norm takes no weights")
-    if not d.rope_dim:
-        _need(positions is None and cos is None and sin is None and pair_axis is None,
-              "a descriptor without rope_dim takes no rotation")
-        return [_ptr(q_weight), _ptr(k_weight), None, None, None, 0, None]
-    if positions is not None and positions.dim() == 1 and d.axes == 1:
-        positions = positions.unsqueeze(0)
-    _ints(positions, (d.axes, d.tokens), "positions")
-    for t, what in ((cos, "cos"), (sin, "sin")):
-        _need(t is not None, f"{what} is required")
-        _need(t.dim() == 2 and t.shape[1] == d.rope_dim // 2 and t.dtype == torch.float32 and t.is_contiguous(),
-              f"{what} must be contiguous f32 [positions, rope_dim / 2]")
-    _need(cos.shape == sin.shape and cos.shape[0] > 0, "cos and sin must have the same rows")
-    if d.axes > 1:
-        _ints(pair_axis, (d.rope_dim // 2,), "pair_axis")
-    else:
-        _need(pair_axis is None, "one axis takes no pair_axis")
-    return [_ptr(q_weight), _ptr(k_weight), _ptr(positions), _ptr(cos), _ptr(sin), cos.shape[0], _ptr(pair_axis)]
+def _pack(tokens=0, hq=0, hk=0, dim=0, rope=0, axes=1, interleaved=False, element=0, norm=False, eps=0.0, ps=0, pages=0,
+          seqs=0, max_q=0, max_kv=0, max_pages=0, causal=False, window=0, scale=0.0, layers=0, page_bytes=0, rows=0) -> bytes:
+    """A plan's sizes as the binding reads them (struct Sizes)."""
+    return struct.pack("9qd8qd3q", tokens, hq, hk, dim, rope, axes, interleaved, element, norm, eps, ps, pages, seqs, max_q,
+                       max_kv, max_pages, causal, window, scale, layers, page_bytes, rows)
 
 
 # ---- norm and rotation -------------------------------------------------------
@@ -119,10 +93,13 @@ class QkNormRopePlan:
     outputs may be the inputs."""
 
     def __init__(self, desc: QkNormRopeDescriptor):
-        self.desc = desc
+        d = self.desc = desc
+        self._packed = _pack(d.tokens, d.num_heads, d.num_kv_heads, d.head_dim, d.rope_dim, d.axes, d.interleaved,
+                             _element(d), d.norm, d.eps)
 
     @classmethod
     def select(cls, desc: QkNormRopeDescriptor) -> "QkNormRopePlan":
+        _sizes_fit(desc)
         check(lib().qk_norm_rope_gfx950_can_implement(desc.tokens, desc.num_heads, desc.num_kv_heads, desc.head_dim,
                                                       desc.rope_dim, desc.axes, _element(desc)),
               "QkNormRopePlan::select")
@@ -134,19 +111,9 @@ class QkNormRopePlan:
 
     def run(self, q, k, q_out, k_out, q_weight=None, k_weight=None, positions=None, cos=None, sin=None,
             pair_axis=None, stream=None) -> None:
-        d = self.desc
-        dtype = _DTYPE[d.element]
-        for t, n, what in ((q, d.num_heads, "q"), (q_out, d.num_heads, "q_out"), (k, d.num_kv_heads, "k"),
-                           (k_out, d.num_kv_heads, "k_out")):
-            _heads(t, d.tokens, n, d.head_dim, dtype, what)
-        _out(q_out, "q_out")
-        _out(k_out, "k_out")
-        _one_device(q, k, q_out, k_out, q_weight, k_weight, positions, cos, sin, pair_axis)
-        rot = _rotation(d, q_weight, k_weight, positions, cos, sin, pair_axis)
-        check(lib().qk_norm_rope_gfx950_run(
-            d.tokens, d.num_heads, d.num_kv_heads, d.head_dim, d.rope_dim, d.axes, int(d.interleaved), _TAG[d.element],
-            d.eps, _ptr(q), *_row(q), _ptr(k), *_row(k), _ptr(q_out), *_row(q_out), _ptr(k_out), *_row(k_out), *rot,
-            _stream(stream)), "QkNormRopePlan::run")
+        st = _kv4.qk_norm_rope(self._packed, stream, q, k, q_out, k_out, q_weight, k_weight, positions, cos, sin, pair_axis)
+        if st:
+            check(st, "QkNormRopePlan::run")
 
 
 # ---- into the cache and back -------------------------------------------------
@@ -166,22 +133,19 @@ class Kv4AppendDescriptor:
     norm: bool = True
 
 
-def _check_cache(cache, d) -> None:
-    _need(cache is not None and cache.dtype == torch.uint8 and cache.is_contiguous() and tuple(cache.shape) ==
-          (d.num_pages, d.num_kv_heads, head_bytes(d.page_size, d.head_dim)),
-          f"cache must be contiguous uint8 [{d.num_pages}, {d.num_kv_heads}, {head_bytes(d.page_size, d.head_dim)}]")
-
-
 class Kv4AppendPlan:
     """K (norm and rotation, rounded to the element) and V of new tokens into
     their slots of the cache, and Q's norm and rotation, in one pass.  K is
     computed in 64 bits, so that the codes are those of the exact values."""
 
     def __init__(self, desc: Kv4AppendDescriptor):
-        self.desc = desc
+        d = self.desc = desc
+        self._packed = _pack(d.tokens, d.num_heads, d.num_kv_heads, d.head_dim, d.rope_dim, d.axes, d.interleaved,
+                             _element(d), d.norm, d.eps, ps=d.page_size, pages=d.num_pages)
 
     @classmethod
     def select(cls, desc: Kv4AppendDescriptor) -> "Kv4AppendPlan":
+        _sizes_fit(desc)
         check(lib().kv4_append_gfx950_can_implement(desc.tokens, desc.num_heads, desc.num_kv_heads, desc.head_dim,
                                                     desc.rope_dim, desc.axes, _element(desc), desc.page_size,
                                                     desc.num_pages), "Kv4AppendPlan::select")
@@ -193,26 +157,10 @@ class Kv4AppendPlan:
 
     def run(self, k, v, cache, slots, q=None, q_out=None, q_weight=None, k_weight=None, positions=None, cos=None,
             sin=None, pair_axis=None, stream=None) -> None:
-        d = self.desc
-        dtype = _DTYPE[d.element]
-        _heads(k, d.tokens, d.num_kv_heads, d.head_dim, dtype, "k")
-        _heads(v, d.tokens, d.num_kv_heads, d.head_dim, dtype, "v")
-        if d.num_heads:
-            _heads(q, d.tokens, d.num_heads, d.head_dim, dtype, "q")
-            _heads(q_out, d.tokens, d.num_heads, d.head_dim, dtype, "q_out")
-            _out(q_out, "q_out")
-        else:
-            _need(q is None and q_out is None, "a descriptor without query heads takes no q")
-        _check_cache(cache, d)
-        _ints(slots, (d.tokens,), "slots", torch.int64)
-        _one_device(q, k, v, q_out, cache, slots, q_weight, k_weight, positions, cos, sin, pair_axis)
-        rot = _rotation(d, q_weight, k_weight, positions, cos, sin, pair_axis)
-        none = (0, 0)
-        check(lib().kv4_append_gfx950_run(
-            d.tokens, d.num_heads, d.num_kv_heads, d.head_dim, d.rope_dim, d.axes, int(d.interleaved), _TAG[d.element],
-            d.eps, d.page_size, d.num_pages, _ptr(q), *(none if q is None else _row(q)), _ptr(k), *_row(k), _ptr(v),
-            *_row(v), _ptr(q_out), *(none if q_out is None else _row(q_out)), _ptr(cache), _ptr(slots), *rot,
-            _stream(stream)), "Kv4AppendPlan::run")
+        st = _kv4.append(self._packed, stream, k, v, cache, slots, q, q_out, q_weight, k_weight, positions, cos, sin,
+                         pair_axis)
+        if st:
+            check(st, "Kv4AppendPlan::run")
 
 
 @dataclass(frozen=True)
@@ -229,10 +177,12 @@ class Kv4ReadPlan:
     """k_out, v_out [tokens, kv heads, D] = the values in the tokens' slots."""
 
     def __init__(self, desc: Kv4ReadDescriptor):
-        self.desc = desc
+        d = self.desc = desc
+        self._packed = _pack(d.tokens, 0, d.num_kv_heads, d.head_dim, element=_element(d), ps=d.page_size, pages=d.num_pages)
 
     @classmethod
     def select(cls, desc: Kv4ReadDescriptor) -> "Kv4ReadPlan":
+        _sizes_fit(desc)
         check(lib().kv4_read_gfx950_can_implement(desc.tokens, desc.num_kv_heads, desc.head_dim, _element(desc),
                                                   desc.page_size, desc.num_pages), "Kv4ReadPlan::select")
         return cls(desc)
@@ -241,16 +191,9 @@ class Kv4ReadPlan:
         return 0
 
     def run(self, cache, slots, k_out, v_out, stream=None) -> None:
-        d = self.desc
-        for t, what in ((k_out, "k_out"), (v_out, "v_out")):
-            _heads(t, d.tokens, d.num_kv_heads, d.head_dim, _DTYPE[d.element], what)
-            _out(t, what)
-        _check_cache(cache, d)
-        _ints(slots, (d.tokens,), "slots", torch.int64)
-        _one_device(cache, slots, k_out, v_out)
-        check(lib().kv4_read_gfx950_run(d.tokens, d.num_kv_heads, d.head_dim, _TAG[d.element], d.page_size, d.num_pages,
-                                        _ptr(cache), _ptr(slots), _ptr(k_out), *_row(k_out), _ptr(v_out), *_row(v_out),
-                                        _stream(stream)), "Kv4ReadPlan::run")
+        st = _kv4.read(self._packed, stream, cache, slots, k_out, v_out)
+        if st:
+            check(st, "Kv4ReadPlan::run")
 
 
 # ---- attention -----------------------------------------------------------------
@@ -277,10 +220,14 @@ class Kv4AttentionPlan:
     tokens are its last ones.  A row that sees nothing gives zeros."""
 
     def __init__(self, desc: Kv4AttentionDescriptor):
-        self.desc = desc
+        d = self.desc = desc
+        self._packed = _pack(d.total_q, d.num_heads, d.num_kv_heads, d.head_dim, element=_element(d), ps=d.page_size,
+                             pages=d.num_pages, seqs=d.num_seqs, max_q=d.max_q, max_kv=d.max_kv, max_pages=d.max_pages,
+                             causal=d.causal, window=d.window, scale=self._sizes(d)[-1])
 
     @classmethod
     def select(cls, desc: Kv4AttentionDescriptor) -> "Kv4AttentionPlan":
+        _sizes_fit(desc)
         check(lib().kv4_attention_gfx950_can_implement(*cls._sizes(desc)), "Kv4AttentionPlan::select")
         return cls(desc)
 
@@ -297,23 +244,9 @@ class Kv4AttentionPlan:
                                                              d.num_kv_heads, d.head_dim, d.window))
 
     def run(self, q, cache, tables, kv_lens, out, cu_q=None, workspace=None, stream=None) -> None:
-        d = self.desc
-        _heads(q, d.total_q, d.num_heads, d.head_dim, _DTYPE[d.element], "q")
-        _heads(out, d.total_q, d.num_heads, d.head_dim, _DTYPE[d.element], "out")
-        _out(out, "out")
-        _check_cache(cache, d)
-        _need(tables is not None and tuple(tables.shape) == (d.num_seqs, d.max_pages) and tables.dtype == torch.int32
-              and (d.max_pages <= 1 or tables.stride(1) == 1), f"tables must be int32 [{d.num_seqs}, {d.max_pages}]")
-        _ints(kv_lens, (d.num_seqs,), "kv_lens")
-        if cu_q is not None:
-            _ints(cu_q, (d.num_seqs + 1,), "cu_q")
-        else:
-            _need(d.max_q == 1 and d.total_q == d.num_seqs, "cu_q is required unless every sequence has one new token")
-        _need(workspace is None or workspace.is_contiguous(), "workspace must be contiguous")
-        _one_device(q, cache, tables, kv_lens, out, cu_q, workspace)
-        check(lib().kv4_attention_gfx950_run(
-            *self._sizes(d), _ptr(q), *_row(q), _ptr(cache), _ptr(tables), tables.stride(0), _ptr(kv_lens), _ptr(cu_q),
-            _ptr(out), *_row(out), _ptr(workspace), _nbytes(workspace), _stream(stream)), "Kv4AttentionPlan::run")
+        st = _kv4.attention(self._packed, stream, q, cache, tables, kv_lens, out, cu_q, workspace)
+        if st:
+            check(st, "Kv4AttentionPlan::run")
 
 
 # ---- pages ---------------------------------------------------------------------
@@ -335,10 +268,13 @@ class KvPagesPlan:
     All of it is on the device, and what a call does is decided there."""
 
     def __init__(self, desc: KvPagesDescriptor):
-        self.desc = desc
+        d = self.desc = desc
+        self._packed = _pack(layers=d.layers, pages=d.num_pages, page_bytes=d.page_bytes, ps=d.page_size, rows=d.rows,
+                             max_pages=d.max_pages)
 
     @classmethod
     def select(cls, desc: KvPagesDescriptor) -> "KvPagesPlan":
+        _sizes_fit(desc)
         check(lib().kv_pages_gfx950_can_implement(*cls._sizes(desc)), "KvPagesPlan::select")
         return cls(desc)
 
@@ -350,76 +286,36 @@ class KvPagesPlan:
         """Bytes that `compact` needs; the other calls need none."""
         return int(lib().kv_pages_gfx950_workspace_size(*self._sizes(self.desc)))
 
-    def _cache(self, cache) -> None:
-        d = self.desc
-        _need(cache is not None and cache.is_contiguous() and cache.element_size() == 1 and
-              tuple(cache.shape) == (d.layers, d.num_pages, d.page_bytes),
-              f"cache must be contiguous bytes [{d.layers}, {d.num_pages}, {d.page_bytes}]")
-
-    def _state(self, tables, lens, refs) -> None:
-        d = self.desc
-        _ints(tables, (d.rows, d.max_pages), "tables")
-        if lens is not None:
-            _ints(lens, (d.rows,), "lens")
-        _ints(refs, (d.num_pages,), "refs")
-
     def copy(self, cache, src, dst, stream=None) -> None:
         """Page src[i] to page dst[i] in every layer; no destination is a source
         or named twice.  Pairs outside the cache are left out."""
-        d = self.desc
-        self._cache(cache)
-        _need(src is not None and src.dim() == 1, "src must be a vector")
-        _ints(src, (src.numel(),), "src")
-        _ints(dst, (src.numel(),), "dst")
-        _one_device(cache, src, dst)
-        check(lib().kv_pages_copy_gfx950_run(d.layers, d.num_pages, d.page_bytes, src.numel(), _ptr(cache), _ptr(src),
-                                             _ptr(dst), _stream(stream)), "KvPagesPlan::copy")
+        st = _kv4.pages_copy(self._packed, stream, cache, src, dst)
+        if st:
+            check(st, "KvPagesPlan::copy")
 
     def fork(self, cache, tables, lens, refs, parents, children, fresh, stream=None) -> None:
         """Row children[i] becomes what row parents[i] is: full pages are shared, a
         partly filled last one is copied to the lowest free page, fresh[i] (-1:
         none was needed; -2, and an empty row: no page was free, or there is no
         such parent).  No child is a parent or holds pages before."""
-        self._cache(cache)
-        self._state(tables, lens, refs)
-        _need(lens is not None, "lens is required")
-        _need(parents is not None and parents.dim() == 1, "parents must be a vector")
-        n = parents.numel()
-        for t, what in ((parents, "parents"), (children, "children"), (fresh, "fresh")):
-            _ints(t, (n,), what)
-        _one_device(cache, tables, lens, refs, parents, children, fresh)
-        check(lib().kv_pages_fork_gfx950_run(*self._sizes(self.desc), n, _ptr(cache), _ptr(tables), _ptr(lens), _ptr(refs),
-                                             _ptr(parents), _ptr(children), _ptr(fresh), _stream(stream)),
-              "KvPagesPlan::fork")
+        st = _kv4.pages_fork(self._packed, stream, cache, tables, lens, refs, parents, children, fresh)
+        if st:
+            check(st, "KvPagesPlan::fork")
 
     def release(self, tables, lens, refs, rows, stream=None) -> None:
         """The rows give their pages back and are empty after."""
-        d = self.desc
-        self._state(tables, lens, refs)
-        _need(lens is not None, "lens is required")
-        _need(rows is not None and rows.dim() == 1, "rows must be a vector")
-        _ints(rows, (rows.numel(),), "rows")
-        _one_device(tables, lens, refs, rows)
-        check(lib().kv_pages_release_gfx950_run(d.num_pages, d.rows, d.max_pages, rows.numel(), _ptr(tables), _ptr(lens),
-                                                _ptr(refs), _ptr(rows), _stream(stream)), "KvPagesPlan::release")
+        st = _kv4.pages_release(self._packed, stream, tables, lens, refs, rows)
+        if st:
+            check(st, "KvPagesPlan::release")
 
     def compact(self, cache, tables, refs, tables_out, refs_out, remap, live, workspace=None, stream=None) -> None:
         """The pages in use move to the front, where live[0] of them lie after:
         the ones past that, lowest first, into the free ones before it, lowest
         first.  remap: each page's new place, -1 for a free one.  tables_out may be
         tables; refs_out is not refs."""
-        d = self.desc
-        self._cache(cache)
-        self._state(tables, None, refs)
-        self._state(tables_out, None, refs_out)
-        _ints(remap, (d.num_pages,), "remap")
-        _ints(live, (1,), "live")
-        _need(refs.data_ptr() != refs_out.data_ptr(), "refs_out must not be refs")
-        _need(workspace is None or workspace.is_contiguous(), "workspace must be contiguous")
-        _one_device(cache, tables, refs, tables_out, refs_out, remap, live, workspace)
-        check(lib().kv_pages_compact_gfx950_run(*self._sizes(d), _ptr(cache), _ptr(tables), _ptr(refs), _ptr(tables_out),
-                                                _ptr(refs_out), _ptr(remap), _ptr(live), _ptr(workspace),
-                                                _nbytes(workspace), _stream(stream)), "KvPagesPlan::compact")
+        st = _kv4.pages_compact(self._packed, stream, cache, tables, refs, tables_out, refs_out, remap, live, workspace)
+        if st:
+            check(st, "KvPagesPlan::compact")
 
 
 __all__ = ["QkNormRopeDescriptor", "QkNormRopePlan", "Kv4AppendDescriptor", "Kv4AppendPlan", "Kv4ReadDescriptor",
