@@ -85,7 +85,9 @@ __global__ __launch_bounds__(64 * NW, OCC) void decode_kernel(const AttnArgs a) 
         if (s.rows <= 0) return;
         part = Part{index, s.lo / 16, s.lo / 16 + tiles_of(s), 1, index};
     }
-    const int t0 = __builtin_amdgcn_readfirstlane(part.t0), t1 = __builtin_amdgcn_readfirstlane(part.t1);
+    s = uniform(s);
+    part = uniform(part);
+    const int t0 = part.t0, t1 = part.t1;
 
     // queries: the right operand, values [g D / 4, (g + 1) D / 4) of row lane % 16
     v4i q[MT][KW];
@@ -115,9 +117,10 @@ __global__ __launch_bounds__(64 * NW, OCC) void decode_kernel(const AttnArgs a) 
     const int32_t *table = a.tables + s.seq * a.table_stride;
     v4f o[MT][OC];
     float m[MT], l[MT];
+    uint32_t poison[MT];           // of a row, the lane's runs that a NaN has reached
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt) {
-        m[mt] = -INFINITY, l[mt] = 0.0f;
+        m[mt] = -INFINITY, l[mt] = 0.0f, poison[mt] = 0;
 #pragma unroll
         for (int c = 0; c < OC; ++c) o[mt][c] = v4f{0, 0, 0, 0};
     }
@@ -146,20 +149,29 @@ __global__ __launch_bounds__(64 * NW, OCC) void decode_kernel(const AttnArgs a) 
             there[n] = held >> n & 1;
             whole = whole && there[n];
         }
+        uint64_t nan[NT][4];   // in a step with masks: the groups of NaN, a run and four tokens a lane
+        bool any_nan = false;
         if (!whole) {
-            // V of tokens that no row sees may be anything, also a NaN, and 0 times it would be one
+            // A weight of 0 keeps neither what lies behind the sequence's end nor a NaN
+            // of a token that only later rows see out of a sum: the one becomes zeros,
+            // the other as well and is given to the rows that see it below.
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
                     const int tok = 16 * (t + n) + 4 * g + j;
-                    if (!there[n] || tok < s.lo || tok >= s.hi) {
+                    const uint32_t byte = 0xffu << (8 * j);
+                    const bool seen = there[n] && tok >= s.lo && tok < s.hi;
+                    const bool odd = (tile[n].vs & byte) == byte;
+                    nan[n][j] = __ballot(seen && odd);
+                    any_nan = any_nan || nan[n][j] != 0;
+                    if (!seen || odd) {
                         constexpr int B = D / 32;   // bytes of a token
                         if constexpr (B == 2) tile[n].v[j / 2] &= j & 1 ? 0x0000ffffu : 0xffff0000u;
                         else
 #pragma unroll
                             for (int w = 0; w < B / 4; ++w) tile[n].v[j * (B / 4) + w] = 0;
-                        tile[n].vs &= ~(0xffu << (8 * j));
+                        tile[n].vs &= ~byte;
                     }
                 }
             }
@@ -197,7 +209,7 @@ __global__ __launch_bounds__(64 * NW, OCC) void decode_kernel(const AttnArgs a) 
                 }
             }
             top = fmaxf(max_over_groups(top) * a.scale, m[mt]);
-            if (__any(top > m[mt])) {
+            if (__any(top > m[mt] + kSlack)) {
                 const float f = top > m[mt] ? exp2_fast(m[mt] - top) : 1.0f;
                 l[mt] *= f;
 #pragma unroll
@@ -240,6 +252,19 @@ __global__ __launch_bounds__(64 * NW, OCC) void decode_kernel(const AttnArgs a) 
                     o[mt][2 * c + 1] = mfma_pv<T>(f, p[mt][n][1], o[mt][2 * c + 1]);
                 }
             }
+        }
+        if (!whole && any_nan) {
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        const int tok = 16 * (t + n) + 4 * k + j;
+                        const uint32_t runs = (uint32_t)(nan[n][j] >> (16 * k + 4 * g)) & 15u;
+#pragma unroll
+                        for (int mt = 0; mt < MT; ++mt) poison[mt] |= tok >= lo[mt] && tok < hi[mt] ? runs : 0u;
+                    }
         }
     };
     const auto held_of = [&](int step) { return __ballot(pages >= 0) >> (step % kAhead * NT) & ((1u << NT) - 1); };
@@ -288,15 +313,15 @@ __global__ __launch_bounds__(64 * NW, OCC) void decode_kernel(const AttnArgs a) 
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
             float *dst = &lds_o[wave][(16 * mt + r) * LD + (4 * g + e) * OC];
+            const float w = poison[mt] >> e & 1 ? NAN : f;
 #pragma unroll
             for (int c = 0; c < OC; c += 4)
-                *(v4f *)(dst + c) = v4f{o[mt][c][e] * f, o[mt][c + 1][e] * f, o[mt][c + 2][e] * f, o[mt][c + 3][e] * f};
+                *(v4f *)(dst + c) = v4f{o[mt][c][e] * w, o[mt][c + 1][e] * w, o[mt][c + 2][e] * w, o[mt][c + 3][e] * w};
         }
     }
     __syncthreads();
-    if (a.slots && part.parts > 1 && blockIdx.x == part.begin * a.hk && threadIdx.x == 0)
+    if (a.slots && blockIdx.x == part.begin * a.hk && threadIdx.x == 0)
         ((int2 *)a.split)[part.item] = make_int2(part.begin, part.parts);
-    if (a.slots && part.parts == 1 && head == 0 && threadIdx.x == 0) ((int2 *)a.split)[part.item] = make_int2(part.begin, 1);
     float *ml = (float *)(a.split + a.part);
     const int64_t all = (int64_t)gridDim.x * RB;
     for (int u = threadIdx.x; u < s.rows * (D / 4); u += 64 * NW) {
@@ -323,6 +348,351 @@ __global__ __launch_bounds__(64 * NW, OCC) void decode_kernel(const AttnArgs a) 
             if (d == 0) ml[2 * at] = top, ml[2 * at + 1] = sum;
             *(v4f *)(ml + 2 * all + at * D + d) = acc;
         }
+    }
+}
+
+// ---- many rows ---------------------------------------------------------------
+typedef float v16f __attribute__((ext_vector_type(16)));
+
+template <typename T>
+__device__ __forceinline__ v16f mfma32(const v4i &a, const v4i &b, const v16f &c) {
+    if constexpr (__is_same(T, Bf16))
+        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, a), __builtin_bit_cast(bf16x8_t, b), c, 0,
+                                                       0, 0);
+    else
+        return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8_t, a), __builtin_bit_cast(f16x8_t, b), c, 0, 0,
+                                                      0);
+}
+
+// Waves of a workgroup, 32 rows each.  Heads of 256 values: the queries and O of
+// 32 rows fill most of 512 registers, so a SIMD has one wave.
+constexpr int prompt_waves(int D) { return D == 256 ? 4 : 8; }
+
+// The 16-byte unit of a row of V^T that holds unit u: rows that are read
+// together and rows that are written together lie in different banks.
+template <int TT>
+__device__ __forceinline__ int v_unit(int d, int u) { return u ^ ((d ^ (d >> 3)) & (TT / 8 - 1)); }
+template <int D>
+__device__ __forceinline__ int k_unit(int tok, int u) { return u ^ (tok & (D == 64 ? 7 : 15)); }
+
+// The item that is `index`-th in line: longest sequence first, its last rows,
+// which see the most tokens, first (more than 64 sequences: in their order).
+__device__ __forceinline__ int item_in_line(const AttnArgs &a, int index) {
+    int seq = index / a.row_blocks;
+    const int block = a.row_blocks - 1 - index % a.row_blocks;
+    if (a.num_seqs > 1 && a.num_seqs <= 64) {
+        const int lane = threadIdx.x & 63;
+        const int len = lane < a.num_seqs ? a.lens[lane] : 0;
+        int rank = 0;
+        for (int j = 0; j < a.num_seqs; ++j) {
+            const int other = __builtin_amdgcn_readlane(len, j);
+            rank += other > len || (other == len && j < lane);
+        }
+        seq = __builtin_ctzll(__ballot(lane < a.num_seqs && rank == seq));
+    }
+    return seq * a.row_blocks + block;
+}
+
+template <typename T, int D>
+__global__ __launch_bounds__(64 * prompt_waves(D), D == 256 ? 1 : 2) void prompt_kernel(const AttnArgs a) {
+    constexpr int KS = D / 16, DB = D / 32, W = D / 32, NW = prompt_waves(D), TT = 16 * NW, ROWS = 32 * NW;
+    __shared__ __align__(16) uint16_t lds_k[TT * D], lds_v[TT * D];
+    __shared__ uint64_t lds_nan[NW][4];
+    __shared__ __align__(8) uint8_t lds_any[NW];   // a wave's tile has such groups
+    __shared__ Part lds_part;
+    __shared__ Item lds_item;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int n = lane & 31, h = lane >> 5;
+    const int head = blockIdx.x % a.hk, index = blockIdx.x / a.hk;
+
+    Part part;
+    Item s;
+    if (a.slots) {
+        if (wave == 0) find_part(a, ROWS, index, lds_part, lds_item);
+        __syncthreads();
+        part = lds_part;
+        if (__builtin_amdgcn_readfirstlane(part.item) < 0) return;
+        s = lds_item;
+    } else {
+        const int item = item_in_line(a, index);
+        s = item_of(a, item, ROWS);
+        if (s.rows <= 0) return;
+        part = Part{item, s.lo / 16, s.lo / 16 + tiles_of(s), 1, index};
+    }
+    s = uniform(s);
+    part = uniform(part);
+    const int t0 = part.t0, t1 = part.t1;
+    const int row = 32 * wave + n;
+    int lo, hi;
+    row_span(a, s, row, lo, hi);
+    // what all of the wave's rows see, and what any of them does
+    const int wave_rows = min(32, s.rows - 32 * wave);
+    int all_lo = 0, all_hi = 0, any_lo = 0, any_hi = 0;
+    if (wave_rows > 0) {
+        row_span(a, s, 32 * wave + wave_rows - 1, all_lo, any_hi);
+        row_span(a, s, 32 * wave, any_lo, all_hi);
+    }
+    v4i q[KS];
+#pragma unroll
+    for (int k = 0; k < KS; ++k) q[k] = v4i{0, 0, 0, 0};
+    const int x = s.first + row;
+    const int64_t x_token = s.q0 + x / a.ratio, x_head = head * a.ratio + x % a.ratio;
+    if (row < s.rows) {
+        const char *p = (const char *)a.q + 2 * (x_token * a.q_token + x_head * a.q_head + 8 * h);
+#pragma unroll
+        for (int k = 0; k < KS; ++k) {
+            const auto m = *(const typename Raw<T>::Mem *)(p + 32 * k);
+            q[k] = v4i{(int)m.w[0], (int)m.w[1], (int)m.w[2], (int)m.w[3]};
+        }
+    }
+
+    // A wave loads and converts 16 of the step's tokens: of K values
+    // [(lane % 4) D / 4, ...) of token lane / 4, of V run lane % 16 of tokens
+    // 4 (lane / 16) ...
+    const int32_t *table = a.tables + s.seq * a.table_stride;
+    // the step that is loaded, and which of its tiles are there
+    uint32_t kw[W], vw[W], ks, vs, next_held = 0;
+    // the pages of 64 / NW steps, a tile a lane
+    int pages = page_of(a, table, t0 + lane, t1), page;
+    const auto load = [&](int t) {
+        if ((t - t0) % 64 == 0 && t > t0) pages = page_of(a, table, t + lane, t1);
+        page = __builtin_amdgcn_readlane(pages, (t - t0) % 64 + wave);
+        next_held = (uint32_t)(__ballot(pages >= 0) >> ((t - t0) % 64)) & ((1u << NW) - 1);
+        const int off = (t + wave) * 16 & (a.ps - 1);
+        const uint8_t *base = a.cache + ((int64_t)(page < 0 ? 0 : page) * a.hk + head) * head_bytes(a.ps, D);
+        load_words(kw, base + off * (D / 2) + lane * (D / 8));
+        load_words(vw, base + v_codes(a.ps, D) + off * (D / 2) + lane * (D / 8));
+        const uint8_t *p = base + k_scales(a.ps, D) + off * (D / 32) + lane * D / 128;
+        ks = D == 256 ? *(const uint16_t *)p : *p;
+        vs = *(const uint32_t *)(base + v_scales(a.ps, D) + (((off >> 2) + (lane >> 4)) * (D / 32) + (lane & 15) * D / 512) * 4);
+    };
+    const auto convert = [&](int t) {
+        uint16_t *lk = lds_k, *lv = lds_v;
+        const int tok = 16 * wave + lane / 4;
+#pragma unroll
+        for (int w = 0; w < W; ++w) {
+            const float sc = scale_bits(D == 256 && w >= 4 ? ks << 15 : ks << 23);
+            v4i f;
+#pragma unroll
+            for (int b = 0; b < 4; ++b) f[b] = (int)pair_of<T>(kw[w], sc, b);
+            *(v4i *)(lk + tok * D + k_unit<D>(tok, lane % 4 * W + w) * 8) = f;
+        }
+        // Tokens that no row sees may hold anything, and a weight of 0 would not
+        // keep a NaN from the other rows either: what is unseen becomes zeros,
+        // groups of NaN are noted and become zeros as well.
+        const int pos = 16 * (t + wave);
+        const bool inside = page >= 0 && pos >= s.lo && pos + 16 <= s.hi;
+        const uint32_t low7 = ~vs & 0x7f7f7f7fu;
+        const bool odd = (((low7 + 0x7f7f7f7fu) | ~vs) & 0x80808080u) != 0x80808080u;   // a byte of 255
+        int any = 0;
+        if (!inside || __any(odd)) {
+            uint64_t nan[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const int at = pos + 4 * (lane >> 4) + j;
+                const uint32_t byte = 0xffu << (8 * j);
+                const bool seen = page >= 0 && at >= s.lo && at < s.hi;
+                nan[j] = __ballot(seen && (vs & byte) == byte);
+                if (!seen || (vs & byte) == byte) {
+                    constexpr int B = D / 32;
+                    if constexpr (B == 2) vw[j / 2] &= j & 1 ? 0x0000ffffu : 0xffff0000u;
+                    else
+#pragma unroll
+                        for (int w = 0; w < B / 4; ++w) vw[j * (B / 4) + w] = 0;
+                    vs &= ~byte;
+                }
+            }
+            any = (nan[0] | nan[1] | nan[2] | nan[3]) != 0;
+            if (any && lane == 0) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) lds_nan[wave][j] = nan[j];
+            }
+        }
+        if (lane == 0) lds_any[wave] = (uint8_t)any;
+        const float sc[4] = {scale_bits(vs << 23), scale_bits(vs << 15), scale_bits(vs << 7), scale_bits(vs >> 1)};
+        // four tokens are 8 bytes of a row of V^T, in the order of the scores' lanes
+        const int g = lane >> 4, unit = 2 * wave + (g & 1), place = 4 * (g >> 1);
+#pragma unroll
+        for (int c = 0; c < D / 32; ++c) {
+            uint32_t w[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const int b = j * (D / 32) + c;
+                w[j] = pair_of<T>(vw[b / 4], sc[j], b % 4);
+            }
+            const int d = (lane & 15) * (D / 16) + 2 * c;
+            *(v2i *)(lv + d * TT + v_unit<TT>(d, unit) * 8 + place) =
+                v2i{(int)__builtin_amdgcn_perm(w[1], w[0], 0x05040100u), (int)__builtin_amdgcn_perm(w[3], w[2], 0x05040100u)};
+            *(v2i *)(lv + (d + 1) * TT + v_unit<TT>(d + 1, unit) * 8 + place) =
+                v2i{(int)__builtin_amdgcn_perm(w[1], w[0], 0x07060302u), (int)__builtin_amdgcn_perm(w[3], w[2], 0x07060302u)};
+        }
+    };
+
+    // where this lane's operands lie: of K unit 2 k + h of token n (32 b + n: an
+    // offset), of V unit 2 k + h of value n, with the block b and d exchanged
+    // by their exclusive or (value 32 d + n, unit 4 b + 2 k + h)
+    int at_k[KS], at_v[2][NW / 2];
+#pragma unroll
+    for (int k = 0; k < KS; ++k) at_k[k] = n * D + k_unit<D>(n, 2 * k + h) * 8;
+#pragma unroll
+    for (int k = 0; k < 2; ++k)
+#pragma unroll
+        for (int e = 0; e < NW / 2; ++e) at_v[k][e] = n * TT + v_unit<TT>(n, 4 * e + 2 * k + h) * 8;
+
+    v16f o[DB];
+#pragma unroll
+    for (int d = 0; d < DB; ++d)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) o[d][i] = 0.0f;
+    float m = -INFINITY, l = 0.0f;
+    uint32_t poison = 0;           // blocks of 32 values that a NaN has reached
+
+    const auto products = [&](int t, uint32_t there) {
+        if (16 * t >= any_hi || 16 * (t + NW) <= any_lo) return;
+        const uint16_t *lk = lds_k, *lv = lds_v;
+        const bool whole = 16 * t >= all_lo && 16 * (t + NW) <= all_hi && there == (1u << NW) - 1;
+        const auto read_k = [&](int b, int k) { return *(const v4i *)(lk + at_k[k] + 32 * b * D); };
+        const auto read_v = [&](int b, int u) {
+            return *(const v4i *)(lv + at_v[u / DB][(b ^ (u % DB)) & (NW / 2 - 1)] + 32 * (u % DB) * TT);
+        };
+        const auto mask = [&](v16f &sc, int b) {
+            float top = -INFINITY;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                const int tok = 16 * t + 32 * b + 8 * (i / 4) + 4 * h + i % 4;
+                if (!(there >> (2 * b + i / 8) & 1) || tok < lo || tok >= hi) sc[i] = -INFINITY;
+                top = fmaxf(top, sc[i]);
+            }
+            return top;
+        };
+        // While the matrix unit has the next block's scores, the vector unit has this
+        // one's weights: an instruction of the one between some of the other, and
+        // operands read two products ahead.
+        constexpr int PV = 2 * DB;
+        v16f sc;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) sc[i] = 0.0f;
+#pragma unroll
+        for (int k = 0; k < KS; ++k) sc = mfma32<T>(read_k(0, k), q[k], sc);
+        float top = sc[0];
+#pragma unroll
+        for (int i = 1; i < 16; ++i) top = fmaxf(top, sc[i]);
+        if (!whole) top = mask(sc, 0);
+#pragma unroll
+        for (int b = 0; b < NW / 2; ++b) {
+            const bool last = b + 1 == NW / 2;
+            const auto both = __builtin_amdgcn_permlane32_swap(__float_as_uint(top), __float_as_uint(top), false, false);
+            top = fmaxf(fmaxf(as_float(both[0]), as_float(both[1])) * a.scale, m);
+            if (__any(top > m + kSlack)) {
+                const float f = top > m ? exp2_fast(m - top) : 1.0f;
+                l *= f;
+#pragma unroll
+                for (int d = 0; d < DB; ++d) o[d] *= f;
+                m = top;
+            }
+            const float ref = m == -INFINITY ? 0.0f : -m;
+            v16f next;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) next[i] = 0.0f;
+            v4i p[2], f[KS], g[PV];
+            if (!last) f[0] = read_k(b + 1, 0), f[1] = read_k(b + 1, 1);
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int k = 0; k < KS; ++k) {
+                if (!last && k + 2 < KS) f[k + 2] = read_k(b + 1, k + 2);
+                if (k + 2 >= KS) g[k + 2 - KS] = read_v(b, k + 2 - KS);
+#pragma unroll
+                for (int x = 8 * k / KS; x < 8 * (k + 1) / KS; ++x) {
+                    const float e0 = exp2_fast(__builtin_fmaf(sc[2 * x], a.scale, ref));
+                    const float e1 = exp2_fast(__builtin_fmaf(sc[2 * x + 1], a.scale, ref));
+                    const uint32_t pair = pack2<T>(e0, e1);
+                    l = add_pair<T>(pair, l);
+                    p[x / 4][x % 4] = (int)pair;
+                }
+                if (!last) next = mfma32<T>(f[k], q[k], next);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+            top = -INFINITY;
+#pragma unroll
+            for (int u = 0; u < PV; ++u) {
+                if (u + 2 < PV) g[u + 2] = read_v(b, u + 2);
+                o[u % DB] = mfma32<T>(g[u], p[u / DB], o[u % DB]);
+                if (!last) {
+#pragma unroll
+                    for (int i = 16 * u / PV; i < 16 * (u + 1) / PV; ++i) top = fmaxf(top, next[i]);
+                }
+                __builtin_amdgcn_sched_barrier(0);
+            }
+            sc = next;
+            if (!last && !whole) top = mask(sc, b + 1);
+        }
+        // groups of NaN, to the rows that see their token
+        uint32_t any = 0;
+#pragma unroll
+        for (int w = 0; w < NW; w += 4) any |= *(const uint32_t *)(lds_any + w);
+        if (__builtin_amdgcn_readfirstlane(any) == 0) return;
+        for (int w = 0; w < NW; ++w) {
+            if (!lds_any[w]) continue;
+            for (int j = 0; j < 4; ++j) {
+                const uint64_t bits = lds_nan[w][j];
+                for (int g = 0; g < 4; ++g) {
+                    const int tok = 16 * (t + w) + 4 * g + j;
+                    const bool seen = tok >= lo && tok < hi;
+#pragma unroll
+                    for (int d = 0; d < DB; ++d)
+                        poison |= seen && (bits >> (16 * g + d * 512 / D) & 1) ? 1u << d : 0u;
+                }
+            }
+        }
+    };
+
+    if (t0 < t1) {
+        load(t0);
+        uint32_t held = next_held;
+        convert(t0);
+        if (t0 + NW < t1) load(t0 + NW);
+        __syncthreads();
+        for (int t = t0; t < t1; t += NW) {
+            products(t, held);
+            __syncthreads();
+            if (t + NW < t1) {
+                held = next_held;
+                convert(t + NW);
+                if (t + 2 * NW < t1) load(t + 2 * NW);
+            }
+            __syncthreads();
+        }
+    }
+    {
+        const auto both = __builtin_amdgcn_permlane32_swap(__float_as_uint(l), __float_as_uint(l), false, false);
+        l = as_float(both[0]) + as_float(both[1]);
+    }
+    if (a.slots && blockIdx.x == part.begin * a.hk && threadIdx.x == 0)
+        ((int2 *)a.split)[part.item] = make_int2(part.begin, part.parts);
+    if (row >= s.rows) return;
+#pragma unroll
+    for (int d = 0; d < DB; ++d)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) o[d][i] += poison >> d & 1 ? NAN : 0.0f;
+    if (part.parts == 1) {
+        const float inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;
+        char *dst = (char *)a.out + 2 * (x_token * a.out_token + x_head * a.out_head + 4 * h);
+        typedef struct __attribute__((packed, aligned(2))) { uint32_t w[2]; } Out;
+#pragma unroll
+        for (int d = 0; d < DB; ++d)
+#pragma unroll
+            for (int i = 0; i < 16; i += 4)
+                *(Out *)(dst + 2 * (32 * d + 2 * i)) =
+                    Out{{pack2<T>(o[d][i] * inv, o[d][i + 1] * inv), pack2<T>(o[d][i + 2] * inv, o[d][i + 3] * inv)}};
+    } else {
+        float *ml = (float *)(a.split + a.part);
+        const int64_t at = (int64_t)blockIdx.x * ROWS + row;
+        if (h == 0) ml[2 * at] = m, ml[2 * at + 1] = l;
+        float *dst = ml + 2 * (int64_t)gridDim.x * ROWS + at * D + 4 * h;
+#pragma unroll
+        for (int d = 0; d < DB; ++d)
+#pragma unroll
+            for (int i = 0; i < 16; i += 4) *(v4f *)(dst + 32 * d + 2 * i) = v4f{o[d][i], o[d][i + 1], o[d][i + 2], o[d][i + 3]};
     }
 }
 
@@ -406,7 +776,7 @@ __global__ __launch_bounds__(256) void join_kernel(const AttnArgs a, int64_t all
 
 // How a problem is cut, the same for the workspace's size and the launch.
 struct Cut {
-    int mt, rows, row_blocks, slots, min_tiles;
+    int rows, row_blocks, slots, min_tiles;
     bool wide;                // one workgroup of many waves has a whole sequence
     int64_t items, grid;
     size_t part, bytes;
@@ -417,16 +787,33 @@ constexpr int kMinTiles = 16;
 constexpr int kJoinWide = 2048;   // rows up to which four waves join one
 constexpr int kWhole = 1024;      // tokens up to which nothing is cut
 
+// Blocks of 32 rows, whose waves share out the tokens, or of 256 (128 for heads of
+// 256 values), whose waves share the converted tokens?  The large blocks have a
+// longer way in and pay where there is work for all CUs: the measure is blocks of
+// 32 rows times tokens.  Large against small, us: heads of 128, 0.8 M 26 and 27,
+// 1.2 M 39 and 38, 2 M 38 and 43, 4.2 M 79 and 111, 24 M 240 and 278; below, 16
+// tokens of 8 heads before 4000 tokens (0.1 M) 23 and 13.  Heads of 256: 0.3 M 40
+// and 29, 0.6 M 47 and 64, 4.2 M 131 and 233.
+bool large_blocks(int64_t blocks, int64_t seen, int D) {
+    return blocks * seen >= (D == 256 ? 500000 : 1500000);
+}
+
 Cut cut_of(int num_seqs, int max_q, int64_t max_kv, int ratio, int hk, int D, int window) {
     Cut c{};
-    c.mt = (int64_t)max_q * ratio <= 16 ? 1 : 2;
-    c.rows = 16 * c.mt;
-    c.row_blocks = (int)(((int64_t)max_q * ratio + c.rows - 1) / c.rows);
-    c.items = (int64_t)num_seqs * c.row_blocks;
+    const int64_t rows = (int64_t)max_q * ratio;
     const int64_t seen = window && window + (int64_t)max_q < max_kv ? window + (int64_t)max_q : max_kv;
-    c.slots = seen <= kWhole || c.items * hk >= 8 * kSlots ? 0 : kSlots;
-    c.min_tiles = kMinTiles;
-    c.wide = !c.slots && c.mt == 1 && seen > 256 && c.items * hk <= 256;
+    const bool large = rows > 32 && large_blocks((rows + 31) / 32 * num_seqs * hk, seen, D);
+    c.rows = rows <= 16 ? 16 : large ? 32 * prompt_waves(D) : 32;
+    c.row_blocks = (int)((rows + c.rows - 1) / c.rows);
+    c.items = (int64_t)num_seqs * c.row_blocks;
+    if (large) {
+        c.slots = seen <= kWhole / 2 || c.items * hk >= kSlots / 2 ? 0 : kSlots / 2;
+        c.min_tiles = 2 * kMinTiles;
+    } else {
+        c.slots = seen <= kWhole || c.items * hk >= 8 * kSlots ? 0 : kSlots;
+        c.min_tiles = kMinTiles;
+    }
+    c.wide = !c.slots && c.rows == 16 && seen > 256 && c.items * hk <= 256;
     c.grid = c.items * hk + c.slots;
     if (c.slots) {
         c.grid = (c.grid + hk - 1) / hk * hk;
@@ -436,11 +823,22 @@ Cut cut_of(int num_seqs, int max_q, int64_t max_kv, int ratio, int hk, int D, in
     return c;
 }
 
+template <typename T, int D, int RB>
+void launch_join(const AttnArgs &a, const Cut &c, hipStream_t stream) {
+    const unsigned items = (unsigned)(c.items * a.hk);
+    if (items * RB <= kJoinWide)
+        hipLaunchKernelGGL((join_kernel<T, D, RB, 4>), dim3(items, RB), dim3(256), 0, stream, a, c.grid * RB);
+    else
+        hipLaunchKernelGGL((join_kernel<T, D, RB, 1>), dim3(items, RB / 4), dim3(256), 0, stream, a, c.grid * RB);
+}
+
 template <typename T, int D>
 int32_t launch_attention(AttnArgs a, const Cut &c, hipStream_t stream) {
     constexpr int WIDE = D == 256 ? 8 : 16, TWO = D == 256 ? 2 : 4;
     const dim3 grid((unsigned)c.grid);
-    if (c.mt == 2)
+    if (c.rows > 32)
+        hipLaunchKernelGGL((prompt_kernel<T, D>), grid, dim3(64 * prompt_waves(D)), 0, stream, a);
+    else if (c.rows == 32)
         hipLaunchKernelGGL((decode_kernel<T, D, 2, 2, TWO, 2>), grid, dim3(64 * TWO), 0, stream, a);
     else if (c.wide)
         hipLaunchKernelGGL((decode_kernel<T, D, 1, 2, WIDE, WIDE / 4>), grid, dim3(64 * WIDE), 0, stream, a);
@@ -448,16 +846,9 @@ int32_t launch_attention(AttnArgs a, const Cut &c, hipStream_t stream) {
         hipLaunchKernelGGL((decode_kernel<T, D, 1, 2, 4, D == 256 ? 2 : 3>), grid, dim3(256), 0, stream, a);
     const int32_t st = launch_status();
     if (st != kOk || !c.slots) return st;
-    const int items = (int)c.items * a.hk;
-    if (items * c.rows <= kJoinWide) {
-        const dim3 grid((unsigned)items, (unsigned)c.rows);
-        if (c.mt == 1) hipLaunchKernelGGL((join_kernel<T, D, 16, 4>), grid, dim3(256), 0, stream, a, c.grid * 16);
-        else hipLaunchKernelGGL((join_kernel<T, D, 32, 4>), grid, dim3(256), 0, stream, a, c.grid * 32);
-    } else {
-        const dim3 grid((unsigned)items, (unsigned)((c.rows + 3) / 4));
-        if (c.mt == 1) hipLaunchKernelGGL((join_kernel<T, D, 16, 1>), grid, dim3(256), 0, stream, a, c.grid * 16);
-        else hipLaunchKernelGGL((join_kernel<T, D, 32, 1>), grid, dim3(256), 0, stream, a, c.grid * 32);
-    }
+    if (c.rows == 16) launch_join<T, D, 16>(a, c, stream);
+    else if (c.rows == 32) launch_join<T, D, 32>(a, c, stream);
+    else launch_join<T, D, 32 * prompt_waves(D)>(a, c, stream);
     return launch_status();
 }
 

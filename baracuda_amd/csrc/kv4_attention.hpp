@@ -152,6 +152,16 @@ __device__ __forceinline__ void find_part(const AttnArgs &a, int block, int inde
     if (lane == 0) part.item = -1;
 }
 
+// The same in scalar registers: all lanes hold the same.
+__device__ __forceinline__ Item uniform(const Item &s) {
+    const auto f = [](int x) { return __builtin_amdgcn_readfirstlane(x); };
+    return Item{f(s.seq), f(s.q0), f(s.first), f(s.rows), f(s.base), f(s.len), f(s.lo), f(s.hi)};
+}
+__device__ __forceinline__ Part uniform(const Part &p) {
+    const auto f = [](int x) { return __builtin_amdgcn_readfirstlane(x); };
+    return Part{f(p.item), f(p.t0), f(p.t1), f(p.parts), f(p.begin)};
+}
+
 template <typename T>
 __device__ __forceinline__ v4f mfma_pv(const v4i &a, const v4i &b, const v4f &c);
 template <>
@@ -198,6 +208,22 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
 // The scale of a conversion: the instruction reads the exponent alone, and 255
 // there makes its results NaN, so the bits around the byte may be anything.
 __device__ __forceinline__ float scale_bits(uint32_t x) { return __uint_as_float(x); }
+
+// l + the two weights of a packed pair, as they are after the rounding.
+template <typename T>
+__device__ __forceinline__ float add_pair(uint32_t pair, float l) {
+    if constexpr (__is_same(T, Bf16)) {
+        typedef __bf16 b2 __attribute__((ext_vector_type(2)));
+        return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(b2, pair), __builtin_bit_cast(b2, 0x3f803f80u), l, false);
+    } else {
+        return __builtin_amdgcn_fdot2(__builtin_bit_cast(f16x2_t, pair), __builtin_bit_cast(f16x2_t, 0x3c003c00u), l, false);
+    }
+}
+
+// How far (in powers of two) a row's maximum may pass the one that its weights
+// are relative to before they are scaled anew: weights stay below 2^8, and most
+// steps need no pass over O.
+constexpr float kSlack = 8.0f;
 
 __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
 

@@ -408,16 +408,69 @@ def test_attention_past_32_bits(gpu, n):
     _same(v[0], want)
 
 
-def test_attention_of_values_that_are_not_finite(gpu):
-    """A NaN that a row sees makes the row NaN; rows before it stay as they are."""
-    lens, qs, d = [64], [6], 128
-    cache, tables, lens_t, cu, q = _scene(torch.Generator().manual_seed(12), lens, qs, 2, 1, d, 16, BF)
-    clean = _attend((cache, tables, lens_t, cu, q), 1).cpu()
+BIG = 2_000_000    # tokens that the host is told of where the large blocks of rows are meant to be taken
+
+
+@pytest.mark.parametrize("part", ["K", "V"])
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("ratio,max_kv", [(1, None), (4, None), (8, None), (8, BIG)], ids=["16 rows", "32 rows", "48 rows", "large"])
+def test_attention_of_values_that_are_not_finite(gpu, part, d, ratio, max_kv):
+    """A NaN that a row sees makes it NaN, in V the values of its group; the rows
+    before it, which do not see it, stay as they are."""
+    lens, qs = [64], [6]
+    cache, tables, lens_t, cu, q = _scene(torch.Generator().manual_seed(12), lens, qs, ratio, 1, d, 16, BF)
+    if part == "V":
+        cache[int(tables[0, 3]), 0, plain.places(16, d)[3][13, 1]] = 127     # so that its place is one of the two before
+    clean = _attend((cache, tables, lens_t, cu, q), 1, max_kv=max_kv).cpu()
     _check_attention(clean, q, cache, tables, lens_t, cu, True, 0, d ** -0.5)
-    ks = plain.places(16, d)[2]
-    cache[int(tables[0, 3]), 0, ks[13]] = 255            # K of token 61, seen by the last three rows
-    got = _attend((cache, tables, lens_t, cu, q), 1).cpu()
-    assert torch.equal(got[:3], clean[:3]) and torch.isnan(got[3:]).all()
+    if part == "K":
+        cache[int(tables[0, 3]), 0, plain.places(16, d)[2][13]] = 255        # token 61, seen by the last three of six
+        got = _attend((cache, tables, lens_t, cu, q), 1, max_kv=max_kv).cpu()
+        assert torch.equal(got[:3], clean[:3]) and torch.isnan(got[3:]).all()
+    else:
+        cache[int(tables[0, 3]), 0, plain.places(16, d)[3][13, 1]] = 255     # values 32 to 63
+        got = _attend((cache, tables, lens_t, cu, q), 1, max_kv=max_kv).cpu()
+        assert torch.equal(got[:3], clean[:3]) and torch.isnan(got[3:, :, 32:64]).all()
+        assert torch.equal(got[3:, :, :32], clean[3:, :, :32]) and torch.equal(got[3:, :, 64:], clean[3:, :, 64:])
+
+
+LARGE = [  # as ATTN, cut into parts by what the host is told
+    ([200, 90, 33], [70, 90, 1], 4, 2, 128, 64, BF, True, 0), ([1100, 150], [300, 20], 2, 1, 64, 16, BF, True, 33),
+    ([140, 70], [40, 3], 5, 5, 128, 16, HF, False, 0), ([40], [64], 4, 2, 64, 16, BF, True, 0),
+    ([600, 130], [257, 129], 8, 2, 256, 64, HF, True, 0), ([1400, 700], [37, 260], 4, 1, 128, 32, BF, True, 500),
+    ([1025] * 3, [17, 1, 33], 16, 2, 128, 32, BF, True, 7), ([129, 128], [128, 127], 2, 2, 256, 128, BF, True, 0)]
+
+
+@pytest.mark.parametrize("case", LARGE, ids=str)
+def test_attention_in_large_blocks(gpu, case):
+    lens, qs, hq, hk, d, ps, dt, causal, window = case
+    print(f"attention {case}", flush=True)
+    scene = _scene(torch.Generator().manual_seed(sum(lens) + d), lens, qs, hq, hk, d, ps, dt)
+    got = _attend(scene, hk, causal, window, max_kv=BIG)
+    cache, tables, lens_t, cu, q = scene
+    _check_attention(got, q, cache, tables, lens_t, cu, causal, window, d ** -0.5)
+    missing = tables.clone()
+    missing[0, 1] = -1
+    got = _attend((cache, missing, lens_t, cu, q), hk, causal, window, max_kv=BIG)
+    _check_attention(got, q, cache, missing, lens_t, cu, causal, window, d ** -0.5)
+
+
+@pytest.mark.parametrize("seqs", [40, 70])
+@pytest.mark.parametrize("most_q", [1, 41])
+@pytest.mark.parametrize("d,told", [(64, 900), (128, 3000), (256, 3000)])
+def test_attention_many_sequences(gpu, seqs, most_q, d, told):
+    """More sequences than a wave has lanes, and more than a round of workgroups; with
+    41 rows blocks of 32, or whole large ones, as the host's bound has it."""
+    rng = random.Random(seqs + most_q)
+    qs = [rng.randint(0, most_q) for _ in range(seqs)]
+    qs[3] = most_q
+    lens = [q + rng.randint(0, 60) for q in qs]
+    lens[5] += 500
+    hk = 8 if most_q > 1 else 2
+    scene = _scene(torch.Generator().manual_seed(seqs), lens, qs, hk, hk, d, 16, BF)
+    got = _attend(scene, hk, max_kv=told)
+    cache, tables, lens_t, cu, q = scene
+    _check_attention(got, q, cache, tables, lens_t, cu, True, 0, d ** -0.5)
 
 
 # ---- pages -----------------------------------------------------------------------
