@@ -101,7 +101,7 @@ __global__ __launch_bounds__(64 * NW, OCC) void decode_kernel(const AttnArgs a) 
         if (row < s.rows) {
             const int x = s.first + row;
             const char *p = (const char *)a.q +
-                            2 * ((s.q0 + x / a.ratio) * a.q_token + (head * a.ratio + x % a.ratio) * a.q_head + g * (D / 4));
+                            2 * ((s.q0 + token_of(a, x)) * a.q_token + (head * a.ratio + x - token_of(a, x) * a.ratio) * a.q_head + g * (D / 4));
 #pragma unroll
             for (int kk = 0; kk < KW; ++kk) {
                 const auto m = *(const typename Raw<T>::Mem *)(p + 16 * kk);
@@ -339,7 +339,7 @@ __global__ __launch_bounds__(64 * NW, OCC) void decode_kernel(const AttnArgs a) 
         if (part.parts == 1) {
             const float inv = sum > 0.0f || sum != sum ? 1.0f / sum : 0.0f;
             const int x = s.first + row;
-            char *dst = (char *)a.out + 2 * ((s.q0 + x / a.ratio) * a.out_token + (head * a.ratio + x % a.ratio) * a.out_head + d);
+            char *dst = (char *)a.out + 2 * ((s.q0 + token_of(a, x)) * a.out_token + (head * a.ratio + x - token_of(a, x) * a.ratio) * a.out_head + d);
             const uint32_t w0 = pack2<T>(acc[0] * inv, acc[1] * inv), w1 = pack2<T>(acc[2] * inv, acc[3] * inv);
             typedef struct __attribute__((packed, aligned(2))) { uint32_t w[2]; } Out;
             *(Out *)dst = Out{{w0, w1}};
@@ -436,7 +436,7 @@ __global__ __launch_bounds__(64 * prompt_waves(D), D == 256 ? 1 : 2) void prompt
 #pragma unroll
     for (int k = 0; k < KS; ++k) q[k] = v4i{0, 0, 0, 0};
     const int x = s.first + row;
-    const int64_t x_token = s.q0 + x / a.ratio, x_head = head * a.ratio + x % a.ratio;
+    const int64_t x_token = s.q0 + token_of(a, x), x_head = head * a.ratio + x - token_of(a, x) * a.ratio;
     if (row < s.rows) {
         const char *p = (const char *)a.q + 2 * (x_token * a.q_token + x_head * a.q_head + 8 * h);
 #pragma unroll
@@ -762,7 +762,7 @@ __global__ __launch_bounds__(256) void join_kernel(const AttnArgs a, int64_t all
     }
     const float inv = sum > 0.0f || sum != sum ? 1.0f / sum : 0.0f;
     const int x = s.first + row;
-    uint16_t *dst = (uint16_t *)a.out + (s.q0 + x / a.ratio) * a.out_token + (head * a.ratio + x % a.ratio) * a.out_head + lane * V;
+    uint16_t *dst = (uint16_t *)a.out + (s.q0 + token_of(a, x)) * a.out_token + (head * a.ratio + x - token_of(a, x) * a.ratio) * a.out_head + lane * V;
     if constexpr (V == 1) {
         dst[0] = (uint16_t)pack2<T>(acc[0] * inv, 0.0f);
     } else {
@@ -914,6 +914,9 @@ extern "C" int32_t baracuda_kernels_kv4_attention_gfx950_run(
     a.split = (char *)workspace, a.part = (int64_t)c.part;
     a.num_seqs = num_seqs, a.total_q = total_q;
     a.hq = num_heads, a.hk = num_kv_heads, a.ratio = num_heads / num_kv_heads;
+    // x magic / 2^32 falls short of the next whole number by less than x ratio / 2^32
+    const uint64_t rows = (uint64_t)max_q * (uint64_t)a.ratio + 512;
+    a.ratio_magic = a.ratio > 1 && rows * (uint64_t)a.ratio < (1ull << 32) ? (uint32_t)(((1ull << 32) + a.ratio - 1) / a.ratio) : 0;
     a.max_pages = max_pages, a.ps = page_size, a.ps_shift = log2i(page_size);
     a.causal = causal != 0, a.window = window;
     a.row_blocks = c.row_blocks, a.items = (int)c.items, a.slots = c.slots, a.min_tiles = c.min_tiles;

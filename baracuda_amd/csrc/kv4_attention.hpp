@@ -23,6 +23,7 @@ struct AttnArgs {
     int64_t q_token, q_head, out_token, out_head, table_stride, num_pages;
     int64_t part;              // bytes from `split` to the partial results
     char *split;               // workspace: int2 per item, then m and l, then O of each part
+    uint32_t ratio_magic;      // ceil(2^32 / ratio) where that divides every row number exactly, else 0
     int num_seqs, total_q, hq, hk, ratio, max_pages, ps, ps_shift, causal, window;
     int row_blocks;            // blocks of rows of a sequence
     int items;                 // num_seqs * row_blocks
@@ -36,9 +37,14 @@ struct Item {
     int seq, q0, first, rows, base, len, lo, hi;
 };
 
+__device__ __forceinline__ int token_of(const AttnArgs &a, int row) {
+    if (a.ratio == 1) return row;
+    return a.ratio_magic ? (int)__umulhi((uint32_t)row, a.ratio_magic) : row / a.ratio;
+}
+
 __device__ __forceinline__ Item item_of(const AttnArgs &a, int item, int block) {
     Item s;
-    s.seq = item / a.row_blocks;
+    s.seq = a.row_blocks == 1 ? item : item / a.row_blocks;
     int q0 = s.seq, n = 1;
     if (a.cu_q) {
         q0 = a.cu_q[s.seq];
@@ -50,11 +56,11 @@ __device__ __forceinline__ Item item_of(const AttnArgs &a, int item, int block) 
     s.q0 = q0;
     s.base = len - n;
     s.len = (int)(len < room ? len : room);
-    s.first = item % a.row_blocks * block;
+    s.first = (item - s.seq * a.row_blocks) * block;
     s.rows = min(block, n * a.ratio - s.first);
     s.lo = s.hi = 0;
     if (s.rows > 0) {
-        const int i0 = s.first / a.ratio, i1 = (s.first + s.rows - 1) / a.ratio;
+        const int i0 = token_of(a, s.first), i1 = token_of(a, s.first + s.rows - 1);
         s.hi = max(0, a.causal ? min(s.len, s.base + i1 + 1) : s.len);
         s.lo = a.window ? max(0, s.base + i0 - a.window + 1) : 0;
     }
@@ -65,7 +71,7 @@ __device__ __forceinline__ int tiles_of(const Item &s) { return s.hi > s.lo ? (s
 
 // The tokens that a row sees: [lo, hi).
 __device__ __forceinline__ void row_span(const AttnArgs &a, const Item &s, int r, int &lo, int &hi) {
-    const int pos = s.base + (s.first + r) / a.ratio;
+    const int pos = s.base + token_of(a, s.first + r);
     const bool in = r < s.rows;
     hi = in ? (a.causal ? min(s.len, pos + 1) : s.len) : 0;
     lo = in && a.window ? max(0, pos - a.window + 1) : 0;
@@ -88,21 +94,16 @@ __device__ __forceinline__ float sum_over_groups(float x) {
     return as_float(b[0]) + as_float(b[1]);
 }
 
-template <typename X>
-__device__ __forceinline__ X wave_sum(X x) {
-#pragma unroll
-    for (int m = 1; m < 64; m *= 2) x += __shfl_xor(x, m, 64);
+// Inclusive sums over the wave's lanes (DPP row shifts and broadcasts).
+__device__ __forceinline__ int wave_scan(int x) {
+    x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, true);    // within rows of 16: 1, 2, 4, 8 lanes up
+    x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, true);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, true);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, true);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false);   // row 0's sum to row 1, row 2's to row 3
+    x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false);   // the first half's to the second
     return x;
 }
-__device__ __forceinline__ float wave_max(float x) {
-#pragma unroll
-    for (int m = 1; m < 64; m *= 2) x = fmaxf(x, __shfl_xor(x, m, 64));
-    return x;
-}
-__device__ __forceinline__ float lane_value(float x, int lane) {
-    return __uint_as_float((uint32_t)__builtin_amdgcn_readlane((int)__float_as_uint(x), lane));
-}
-
 // A part of an item: tiles [t0, t1) of 16 tokens.  `parts` parts have the item,
 // the first of them is part `begin` of all.
 struct Part {
@@ -122,7 +123,7 @@ __device__ __forceinline__ void find_part(const AttnArgs &a, int block, int inde
         if (i0 + lane < a.items) s = item_of(a, i0 + lane, block);
         total += tiles_of(s);
     }
-    total = wave_sum(total);
+    total = __builtin_amdgcn_readlane(wave_scan(total), 63);
     const int per = max(a.min_tiles, (int)(((int64_t)total * a.hk + a.slots - 1) / a.slots));
     int begin = 0;
     for (int i0 = 0; i0 < a.items; i0 += 64) {
@@ -132,12 +133,7 @@ __device__ __forceinline__ void find_part(const AttnArgs &a, int block, int inde
         }
         const int tiles = tiles_of(s);
         const int n = s.rows > 0 ? max(1, (tiles + per - 1) / per) : 0;
-        int sum = n;
-#pragma unroll
-        for (int d = 1; d < 64; d *= 2) {
-            const int o = __shfl_up(sum, d, 64);
-            if (lane >= d) sum += o;
-        }
+        const int sum = wave_scan(n);
         const int mine = begin + sum - n;
         const bool hit = index >= mine && index < mine + n;
         if (hit) {
@@ -147,7 +143,7 @@ __device__ __forceinline__ void find_part(const AttnArgs &a, int block, int inde
             item = s;
         }
         if (__any(hit)) return;
-        begin += __shfl(sum, 63, 64);
+        begin += __builtin_amdgcn_readlane(sum, 63);
     }
     if (lane == 0) part.item = -1;
 }

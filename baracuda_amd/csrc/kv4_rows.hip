@@ -27,6 +27,8 @@ namespace {
 using namespace kv4;
 
 constexpr int kWaves = 4;
+constexpr int kIters = 6;          // rounds of heads of a wave where there are many tokens
+constexpr int64_t kManyTokens = 512;
 
 struct RowArgs {
     const void *src[3];        // Q, K, V
@@ -42,15 +44,9 @@ struct RowArgs {
     const int64_t *slots;
     int64_t num_slots;
     double eps;
+    float inv_D;
     int hq, hk, D, rope, axes, ps, ps_shift, most;
 };
-
-template <typename A>
-__device__ __forceinline__ A inv_root(A x);
-template <>
-__device__ __forceinline__ float inv_root<float>(float x) { return 1.0f / __builtin_sqrtf(x); }
-template <>
-__device__ __forceinline__ double inv_root<double>(double x) { return 1.0 / __builtin_sqrt(x); }
 
 // Lane exchanges within the G lanes of a head, for a sum: after step k all
 // lanes of 2^(k+1) hold the same, so a mirrored lane serves as well as the one
@@ -92,53 +88,31 @@ __device__ __forceinline__ A head_sum(A x) {
     return x;
 }
 
-// The norm and the rotation of one head in type A: eight values a lane (x), the
-// other sides of their pairs (z) and both sides' weights.
-template <typename A, int G>
-__device__ __forceinline__ void norm_rope(const float (&x)[8], const float (&z)[8], float (&y)[8], const float (&w)[8],
-                                          const float (&wz)[8], bool norm, double eps, int D, bool turn, const float (&c)[8],
-                                          const float (&s)[8]) {
-    A r = 1;
-    if (norm) {
-        A sum = 0;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) sum = __builtin_elementwise_fma((A)x[i], (A)x[i], sum);
-        r = inv_root<A>(head_sum<A, G>(sum) / (A)D + (A)eps);
-    }
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        A v = (A)x[i], o = (A)z[i];
-        if (norm) v = v * r * (A)w[i], o = o * r * (A)wz[i];
-        const A t = __builtin_elementwise_fma(v, (A)c[i], o * (A)s[i]);
-        y[i] = (float)(turn ? t : v);
-    }
-}
-
-// G lanes a head, ITERS heads a lane, `share` of the workgroup's waves a token.
-// T: the element; KV4: K and V go into the cache.
+// G lanes a head, ITERS rounds of 64 / G heads a wave, `share` of the workgroup's
+// waves a token.  A round has heads of one kind (Q, K or V), so what differs
+// between them is scalar.  T: the element; KV4: K and V go into the cache.
 template <typename T, int G, int ITERS, bool KV4>
 __global__ __launch_bounds__(64 * kWaves) void rows_kernel(const RowArgs a, int share, bool inter) {
     typedef typename Raw<T>::Mem Mem;
-    constexpr int HPW = 64 / G, W = sizeof(Mem) / 4;
+    constexpr int HPW = 64 / G, W = sizeof(Mem) / 4, SIZE = sizeof(Mem) / 8;
     __shared__ __align__(16) float lds_c[kWaves][128], lds_s[kWaves][128];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int64_t token = (int64_t)blockIdx.x * (kWaves / share) + wave / share;
-    const int l = lane % G, at = 8 * l;
-    const int heads = a.hq + a.hk * (KV4 ? 2 : 1);
-    const int first = (blockIdx.y * share + wave % share) * HPW * ITERS + lane / G;
-    const bool here = token < a.tokens, mine = here && at < a.D;
+    const int l = lane % G, at = 8 * l, sub = lane / G;
+    const int rq = (a.hq + HPW - 1) / HPW, rk = (a.hk + HPW - 1) / HPW, rounds = rq + rk * (KV4 ? 2 : 1);
+    const int first = (blockIdx.y * share + wave % share) * ITERS;
+    const bool here = token < a.tokens;
+    const auto kind_of = [&](int r) { return r < rq ? 0 : r < rq + rk ? 1 : 2; };
+    const auto head_of = [&](int r, int kind) { return (r - (kind == 0 ? 0 : kind == 1 ? rq : rq + rk)) * HPW + sub; };
 
     Mem raw[ITERS];
 #pragma unroll
     for (int it = 0; it < ITERS; ++it) {
-        const int h = first + it * HPW;
-        const int kind = h < a.hq ? 0 : h < a.hq + a.hk ? 1 : 2;
-        const int hh = h - (kind == 0 ? 0 : kind == 1 ? a.hq : a.hq + a.hk);
         raw[it] = Mem{};
-        if (mine && h < heads) {
-            const int64_t off = token * a.src_token[kind] + hh * a.src_head[kind] + at;
-            raw[it] = *(const Mem *)((const char *)a.src[kind] + off * (int64_t)(sizeof(Mem) / 8));
-        }
+        const int r = first + it, kind = kind_of(r), head = head_of(r, kind);
+        if (here && r < rounds && at < a.D && head < (kind ? a.hk : a.hq))
+            raw[it] = *(const Mem *)((const char *)a.src[kind] +
+                                     (token * a.src_token[kind] + head * a.src_head[kind] + at) * SIZE);
     }
 
     // the token's cosines and sines, once for all its heads, through LDS
@@ -154,28 +128,19 @@ __global__ __launch_bounds__(64 * kWaves) void rows_kernel(const RowArgs a, int 
             ls[p] = ok ? a.sine[row * half + p] : 0.0f;
         }
     }
+    int64_t slot = 0;
+    if constexpr (KV4) slot = here ? a.slots[token] : -1;
+    __syncthreads();
+    if (!here) return;
 
     // this lane's, the sine with the sign of its side, and the lane that holds
     // the other side of its pairs (its own when interleaved)
     const bool turn = at < a.rope, low = at < half;
     const int other = inter || !turn ? l : low ? l + half / 8 : l - half / 8;
     const bool norm = a.weight[0] != nullptr;
-    float w[2][8], wz[2][8];
-#pragma unroll
-    for (int k = 0; k < 2; ++k) {
-        Mem m{}, z{};
-        if (norm && at < a.D) {
-            m = *(const Mem *)((const char *)a.weight[k] + (int64_t)at * (sizeof(Mem) / 8));
-            z = *(const Mem *)((const char *)a.weight[k] + (int64_t)(8 * other) * (sizeof(Mem) / 8));
-        }
-#pragma unroll
-        for (int i = 0; i < 8; ++i) w[k][i] = Raw<T>::get(m, i), wz[k][i] = Raw<T>::get(z, inter ? i ^ 1 : i);
-    }
-    int64_t slot = 0;
-    if constexpr (KV4) slot = here ? a.slots[token] : -1;
-    __syncthreads();
-    if (!here) return;
     float c[8], s[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) c[i] = 1.0f, s[i] = 0.0f;
     if (turn) {
         const int p0 = inter ? at / 2 : low ? at : at - half;
 #pragma unroll
@@ -185,42 +150,77 @@ __global__ __launch_bounds__(64 * kWaves) void rows_kernel(const RowArgs a, int 
             s[i] = (inter ? (i & 1) == 0 : low) ? -ls[p] : ls[p];
         }
     }
+    // the weights of both sides, and their products with cosine and sine
+    Mem mw{}, mz{};
+    float cw[8], sw[8];
+    int held = -1;
 
 #pragma unroll
     for (int it = 0; it < ITERS; ++it) {
-        const int h = first + it * HPW;
-        if (h - lane / G >= heads) break;
-        const int kind = h < a.hq ? 0 : h < a.hq + a.hk ? 1 : 2;
-        const int hh = h - (kind == 0 ? 0 : kind == 1 ? a.hq : a.hq + a.hk);
+        const int r = first + it;
+        if (r >= rounds) break;
+        const int kind = kind_of(r), head = head_of(r, kind);
+        const bool mine = at < a.D && head < (kind ? a.hk : a.hq);
+        if (norm && kind < 2 && kind != held) {
+            held = kind;
+            if (at < a.D) {
+                mw = *(const Mem *)((const char *)a.weight[kind] + at * SIZE);
+                mz = *(const Mem *)((const char *)a.weight[kind] + 8 * other * SIZE);
+            }
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                cw[i] = c[i] * Raw<T>::get(mw, i);
+                sw[i] = s[i] * Raw<T>::get(mz, inter ? i ^ 1 : i);
+            }
+        }
         float x[8], z[8], y[8];
 #pragma unroll
         for (int i = 0; i < 8; ++i) x[i] = Raw<T>::get(raw[it], i);
-        if (inter) {
+        if (kind < 2) {
+            if (inter) {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) z[i] = x[i ^ 1];
-        } else {
-            Mem m;
+                for (int i = 0; i < 8; ++i) z[i] = turn ? x[i ^ 1] : 0.0f;
+            } else {
+                Mem m;
 #pragma unroll
-            for (int i = 0; i < W; ++i) m.w[i] = (uint32_t)__shfl((int)raw[it].w[i], other, G);
+                for (int i = 0; i < W; ++i) m.w[i] = (uint32_t)__shfl((int)raw[it].w[i], other, G);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) z[i] = Raw<T>::get(m, i);
+                for (int i = 0; i < 8; ++i) z[i] = Raw<T>::get(m, i);
+            }
         }
         if (!KV4 || kind == 0) {
-            float wh[8], wo[8];
+            if (norm) {
+                float sum = 0;
 #pragma unroll
-            for (int i = 0; i < 8; ++i) wh[i] = w[KV4 ? 0 : kind == 1][i], wo[i] = wz[KV4 ? 0 : kind == 1][i];
-            norm_rope<float, G>(x, z, y, wh, wo, norm, a.eps, a.D, turn, c, s);
-            if (mine && h < heads) {
+                for (int i = 0; i < 8; ++i) sum = __builtin_fmaf(x[i], x[i], sum);
+                const float root = __builtin_amdgcn_rsqf(__builtin_fmaf(head_sum<float, G>(sum), a.inv_D, (float)a.eps));
+#pragma unroll
+                for (int i = 0; i < 8; ++i) y[i] = root * __builtin_fmaf(z[i], sw[i], x[i] * cw[i]);
+            } else {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) y[i] = turn ? __builtin_fmaf(z[i], s[i], x[i] * c[i]) : x[i];
+            }
+            if (mine) {
                 Mem out;
                 Raw<T>::put(out, y);
-                const int64_t off = token * a.dst_token[kind] + hh * a.dst_head[kind] + at;
-                *(Mem *)((char *)a.dst[kind] + off * (int64_t)(sizeof(Mem) / 8)) = out;
+                *(Mem *)((char *)a.dst[kind] + (token * a.dst_token[kind] + head * a.dst_head[kind] + at) * SIZE) = out;
             }
         } else if constexpr (KV4) {
             if (kind == 1) {
-                norm_rope<double, G>(x, z, y, w[1], wz[1], norm, a.eps, a.D, turn, c, s);
+                double root = 1;
+                if (norm) {
+                    double sum = 0;
 #pragma unroll
-                for (int i = 0; i < 8; ++i) y[i] = Raw<T>::round(y[i]);
+                    for (int i = 0; i < 8; ++i) sum += (double)(x[i] * x[i]);   // 22 bits at most: exact
+                    root = 1.0 / __builtin_sqrt(head_sum<double, G>(sum) / (double)a.D + a.eps);
+                }
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    float v = x[i], o = z[i];
+                    if (norm) v *= Raw<T>::get(mw, i), o *= Raw<T>::get(mz, inter ? i ^ 1 : i);   // exact as well
+                    const double t = turn ? __builtin_fma((double)v, (double)c[i], (double)o * (double)s[i]) : (double)v;
+                    y[i] = Raw<T>::round((float)(t * root));
+                }
             } else {
 #pragma unroll
                 for (int i = 0; i < 8; ++i) y[i] = x[i];
@@ -234,9 +234,9 @@ __global__ __launch_bounds__(64 * kWaves) void rows_kernel(const RowArgs a, int 
             const bool good = top < 0x7f800000u;
             const int byte = good ? scale_byte(top, a.most) : 255;
             const uint32_t code = good ? encode8(y, byte) : 0u;
-            if (mine && h < heads && slot >= 0 && slot < a.num_slots) {
+            if (mine && slot >= 0 && slot < a.num_slots) {
                 const int off = (int)(slot & (a.ps - 1)), few = a.D / 32;
-                uint8_t *base = a.cache + ((slot >> a.ps_shift) * a.hk + hh) * head_bytes(a.ps, a.D);
+                uint8_t *base = a.cache + ((slot >> a.ps_shift) * a.hk + head) * head_bytes(a.ps, a.D);
                 if (kind == 1) {
                     *(uint32_t *)(base + off * (a.D / 2) + 4 * l) = code;
                     if (l % 4 == 0) base[k_scales(a.ps, a.D) + off * few + l / 4] = (uint8_t)byte;
@@ -302,14 +302,13 @@ __global__ __launch_bounds__(256) void read_kernel(const uint8_t *__restrict__ c
 
 template <typename T, int G, bool KV4>
 void launch_lanes(const RowArgs &a, bool inter, hipStream_t stream) {
-    const int heads = a.hq + a.hk * (KV4 ? 2 : 1), rounds = (heads + 64 / G - 1) / (64 / G);
-    // a wave has up to three rounds of heads of a token where there are tokens
-    // enough to fill the card without cutting them finer
-    const int iters = rounds > 2 * kWaves && a.tokens >= 512 ? 3 : 1;
+    constexpr int HPW = 64 / G;
+    const int rounds = (a.hq + HPW - 1) / HPW + (a.hk + HPW - 1) / HPW * (KV4 ? 2 : 1);
+    const int iters = a.tokens >= kManyTokens ? kIters : 1;
     const int waves = (rounds + iters - 1) / iters;
     const int share = waves >= 3 ? 4 : waves;
     const dim3 grid((unsigned)((a.tokens + kWaves / share - 1) / (kWaves / share)), (unsigned)((waves + share - 1) / share));
-    if (iters == 3) hipLaunchKernelGGL((rows_kernel<T, G, 3, KV4>), grid, dim3(64 * kWaves), 0, stream, a, share, inter);
+    if (iters > 1) hipLaunchKernelGGL((rows_kernel<T, G, kIters, KV4>), grid, dim3(64 * kWaves), 0, stream, a, share, inter);
     else hipLaunchKernelGGL((rows_kernel<T, G, 1, KV4>), grid, dim3(64 * kWaves), 0, stream, a, share, inter);
 }
 
@@ -373,7 +372,7 @@ extern "C" int32_t baracuda_kernels_qk_norm_rope_gfx950_run(
     a.weight[0] = q_weight, a.weight[1] = k_weight;
     a.positions = positions, a.cosine = cosine, a.sine = sine;
     a.pair_axis = axes > 1 ? pair_axis : nullptr;
-    a.tokens = tokens, a.table_rows = table_rows, a.eps = eps;
+    a.tokens = tokens, a.table_rows = table_rows, a.eps = eps, a.inv_D = 1.0f / (float)head_dim;
     a.hq = num_heads, a.hk = num_kv_heads, a.D = head_dim, a.rope = rope_dim, a.axes = axes;
     const hipStream_t s = (hipStream_t)stream;
     if (element == kF32) return launch_style<float, false>(a, interleaved != 0, s);
@@ -415,7 +414,7 @@ extern "C" int32_t baracuda_kernels_kv4_append_gfx950_run(
     a.weight[0] = q_weight, a.weight[1] = k_weight;
     a.positions = positions, a.cosine = cosine, a.sine = sine;
     a.pair_axis = axes > 1 ? pair_axis : nullptr;
-    a.tokens = tokens, a.table_rows = table_rows, a.eps = eps;
+    a.tokens = tokens, a.table_rows = table_rows, a.eps = eps, a.inv_D = 1.0f / (float)head_dim;
     a.hq = num_heads, a.hk = num_kv_heads, a.D = head_dim, a.rope = rope_dim, a.axes = axes;
     a.cache = (uint8_t *)cache, a.slots = slots, a.num_slots = num_pages * page_size;
     a.ps = page_size, a.ps_shift = log2i(page_size), a.most = element == kF16 ? 13 : 125;
