@@ -59,8 +59,9 @@ __device__ __forceinline__ int page_of(const AttnArgs &a, const int32_t *row, in
     return p >= 0 && p < a.num_pages ? p : -1;
 }
 
-// MT tiles of 16 rows; NT tiles of 16 tokens a step; NW waves.
-template <typename T, int D, int MT, int NT, int NW, int OCC>
+// MT tiles of 16 rows; NT tiles of 16 tokens a step; NW waves; AHEAD: the next
+// step's loads go out before this one's products.
+template <typename T, int D, int MT, int NT, int NW, int OCC, bool AHEAD = true>
 __global__ __launch_bounds__(64 * NW, OCC) void decode_kernel(const AttnArgs a) {
     constexpr int RB = 16 * MT, KW = D / 32, OC = D / 16;
     constexpr int LD = D + 4;
@@ -268,7 +269,7 @@ __global__ __launch_bounds__(64 * NW, OCC) void decode_kernel(const AttnArgs a) 
         }
     };
     const auto held_of = [&](int step) { return __ballot(pages >= 0) >> (step % kAhead * NT) & ((1u << NT) - 1); };
-    if constexpr (NW >= 8) {
+    if constexpr (!AHEAD) {
         for (int i = 0; i < steps; ++i) {
             if (i && i % kAhead == 0) pages = pages_from(i);
             Tile<D> tile[NT];
@@ -276,7 +277,6 @@ __global__ __launch_bounds__(64 * NW, OCC) void decode_kernel(const AttnArgs a) 
             do_step(tile, t0 + i * (NW * NT) + wave * NT, held_of(i));
         }
     } else if (steps) {
-        // the next step's loads go out before this one's products
         Tile<D> even[NT], odd[NT];
         load_step(even, 0);
         uint64_t held = held_of(0);
@@ -785,7 +785,13 @@ struct Cut {
 constexpr int kSlots = 512;
 constexpr int kMinTiles = 16;
 constexpr int kJoinWide = 2048;   // rows up to which four waves join one
-constexpr int kWhole = 1024;      // tokens up to which nothing is cut
+
+// Tokens up to which one workgroup of eight waves takes a sequence whole: parts
+// and their join cost a second launch.  One row, 8 kv heads, whole against cut,
+// us: heads of 128, 1100 tokens 10.0 and 12.0, 2000 14.9 and 12.1; of 64, 2000 12.5
+// and 12.3; of 256, 1100 12.8 and 12.6.  (Blocks of 32 rows have four waves: 1030
+// tokens 15.6 and 13.4.)
+constexpr int whole_tokens(int D, int rows) { return rows > 16 || D == 256 ? 1024 : D == 128 ? 1280 : 1792; }
 
 // Blocks of 32 rows, whose waves share out the tokens, or of 256 (128 for heads of
 // 256 values), whose waves share the converted tokens?  The large blocks have a
@@ -807,10 +813,10 @@ Cut cut_of(int num_seqs, int max_q, int64_t max_kv, int ratio, int hk, int D, in
     c.row_blocks = (int)((rows + c.rows - 1) / c.rows);
     c.items = (int64_t)num_seqs * c.row_blocks;
     if (large) {
-        c.slots = seen <= kWhole / 2 || c.items * hk >= kSlots / 2 ? 0 : kSlots / 2;
+        c.slots = seen <= 512 || c.items * hk >= kSlots / 2 ? 0 : kSlots / 2;
         c.min_tiles = 2 * kMinTiles;
     } else {
-        c.slots = seen <= kWhole || c.items * hk >= 8 * kSlots ? 0 : kSlots;
+        c.slots = seen <= whole_tokens(D, c.rows) || c.items * hk >= 8 * kSlots ? 0 : kSlots;
         c.min_tiles = kMinTiles;
     }
     c.wide = !c.slots && c.rows == 16 && seen > 256 && c.items * hk <= 256;
@@ -834,14 +840,14 @@ void launch_join(const AttnArgs &a, const Cut &c, hipStream_t stream) {
 
 template <typename T, int D>
 int32_t launch_attention(AttnArgs a, const Cut &c, hipStream_t stream) {
-    constexpr int WIDE = D == 256 ? 8 : 16, TWO = D == 256 ? 2 : 4;
+    constexpr int TWO = D == 256 ? 2 : 4;
     const dim3 grid((unsigned)c.grid);
     if (c.rows > 32)
         hipLaunchKernelGGL((prompt_kernel<T, D>), grid, dim3(64 * prompt_waves(D)), 0, stream, a);
     else if (c.rows == 32)
         hipLaunchKernelGGL((decode_kernel<T, D, 2, 2, TWO, 2>), grid, dim3(64 * TWO), 0, stream, a);
     else if (c.wide)
-        hipLaunchKernelGGL((decode_kernel<T, D, 1, 2, WIDE, WIDE / 4>), grid, dim3(64 * WIDE), 0, stream, a);
+        hipLaunchKernelGGL((decode_kernel<T, D, 1, 2, 8, 2, D != 256>), grid, dim3(512), 0, stream, a);
     else
         hipLaunchKernelGGL((decode_kernel<T, D, 1, 2, 4, D == 256 ? 2 : 3>), grid, dim3(256), 0, stream, a);
     const int32_t st = launch_status();
