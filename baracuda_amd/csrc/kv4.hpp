@@ -27,6 +27,12 @@ __host__ __device__ inline int v_codes(int ps, int D) { return ps * D / 2; }
 __host__ __device__ inline int k_scales(int ps, int D) { return ps * D; }
 __host__ __device__ inline int v_scales(int ps, int D) { return ps * D + ps * D / 32; }
 
+// Two f32 -> packed f16x2, each rounded to nearest even.
+typedef _Float16 f16x2_t __attribute__((ext_vector_type(2)));
+__device__ __forceinline__ uint32_t f32x2_to_f16x2(float lo, float hi) {
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2_t){lo, hi}, f16x2_t));
+}
+
 inline bool page_size_ok(int ps) { return ps >= 16 && ps <= 1024 && (ps & (ps - 1)) == 0; }
 inline bool head_dim_ok(int D) { return D == 64 || D == 128 || D == 256; }
 inline int log2i(int x) { return 31 - __builtin_clz((unsigned)x); }
@@ -66,8 +72,7 @@ struct Raw<F16> {
     }
     static __device__ __forceinline__ void put(Mem &m, const float (&x)[8]) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-            m.w[i] = (uint32_t)f32_to_f16_rne(x[2 * i]) | (uint32_t)f32_to_f16_rne(x[2 * i + 1]) << 16;
+        for (int i = 0; i < 4; ++i) m.w[i] = f32x2_to_f16x2(x[2 * i], x[2 * i + 1]);
     }
     static __device__ __forceinline__ float round(float x) { return (float)(_Float16)x; }
 };
@@ -92,25 +97,14 @@ __device__ __forceinline__ uint32_t encode8(const float (&x)[8], int byte) {
     return w;
 }
 
-// A scale byte as the power of two that it stands for; 255 is a NaN.
-__device__ __forceinline__ float scale_value(uint32_t byte) {
-    return __uint_as_float(byte == 255u ? 0x7fc00000u : byte << 23);
-}
-
+// Eight values from their codes and scale byte.  The conversion reads the scale's
+// exponent alone, and 255 there gives NaN.
 __device__ __forceinline__ void decode8(uint32_t w, uint32_t byte, float (&x)[8]) {
     const float s = __uint_as_float(byte << 23);
+    const f32x2_t p[4] = {__builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, s, 0), __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, s, 1),
+                          __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, s, 2), __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, s, 3)};
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        f32x2_t p;
-        switch (i) {
-            case 0: p = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, s, 0); break;
-            case 1: p = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, s, 1); break;
-            case 2: p = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, s, 2); break;
-            default: p = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, s, 3); break;
-        }
-        x[2 * i] = byte == 255u ? __uint_as_float(0x7fc00000u) : p[0];
-        x[2 * i + 1] = byte == 255u ? __uint_as_float(0x7fc00000u) : p[1];
-    }
+    for (int i = 0; i < 4; ++i) x[2 * i] = p[i][0], x[2 * i + 1] = p[i][1];
 }
 
 }  // namespace kv4

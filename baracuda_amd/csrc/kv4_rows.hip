@@ -257,20 +257,28 @@ __global__ __launch_bounds__(64 * kWaves) void rows_kernel(const RowArgs a, int 
     }
 }
 
-// A lane reads eight values of K or V of one token; slots out of range read as zeros.
+// A lane reads eight values of K or V of one token; slots out of range read as
+// zeros.  A workgroup has `several` tokens, or part of one.
 template <typename T>
 __global__ __launch_bounds__(256) void read_kernel(const uint8_t *__restrict__ cache, const int64_t *__restrict__ slots,
-                                                   int64_t num_slots, void *k_out, int64_t k_token, int64_t k_head,
-                                                   void *v_out, int64_t v_token, int64_t v_head, int hk, int D, int ps,
-                                                   int ps_shift) {
+                                                   int64_t tokens, int64_t num_slots, void *k_out, int64_t k_token,
+                                                   int64_t k_head, void *v_out, int64_t v_token, int64_t v_head, int hk,
+                                                   int lane_shift, int ps, int ps_shift, int several) {
     typedef typename Raw<T>::Mem Mem;
-    const int64_t token = blockIdx.x;
-    const int lanes = D / 8, few = D / 32;
+    const int lanes = 1 << lane_shift, D = 8 * lanes, few = D / 32, units = 2 * hk * lanes;
+    int64_t token = blockIdx.x;
+    int first = blockIdx.y * blockDim.x + threadIdx.x;
+    if (several > 1) {
+        const int mine = first / units;
+        token = token * several + mine;
+        first -= mine * units;
+        if (mine >= several || token >= tokens) return;
+    }
     const int64_t slot = slots[token];
     const bool in = slot >= 0 && slot < num_slots;
     const int off = (int)(slot & (ps - 1));
-    for (int u = blockIdx.y * blockDim.x + threadIdx.x; u < 2 * hk * lanes; u += gridDim.y * blockDim.x) {
-        const int l = u % lanes, row = u / lanes;
+    for (int u = first; u < units; u += gridDim.y * blockDim.x) {
+        const int l = u & (lanes - 1), row = u >> lane_shift;
         const bool is_v = row >= hk;
         const int h = is_v ? row - hk : row;
         uint32_t code = 0, byte = 0;
@@ -442,20 +450,15 @@ extern "C" int32_t baracuda_kernels_kv4_read_gfx950_run(
     if (tokens == 0) return kOk;
     if (!cache || !slots || !k_out || !v_out) return kInvalid;
     if (!aligned(k_out, element) || !aligned(v_out, element) || ((uintptr_t)cache & 15u)) return kMisaligned;
-    const int units = 2 * num_kv_heads * (head_dim / 8);
-    const dim3 grid((unsigned)tokens, (unsigned)((units + 255) / 256 < 4 ? (units + 255) / 256 : 4));
-    const hipStream_t s = (hipStream_t)stream;
-    const uint8_t *c = (const uint8_t *)cache;
-    const int64_t n = num_pages * page_size;
-    const int sh = log2i(page_size);
-    if (element == kF32)
-        hipLaunchKernelGGL((read_kernel<float>), grid, dim3(256), 0, s, c, slots, n, k_out, k_token_stride,
-                           k_head_stride, v_out, v_token_stride, v_head_stride, num_kv_heads, head_dim, page_size, sh);
-    else if (element == kF16)
-        hipLaunchKernelGGL((read_kernel<F16>), grid, dim3(256), 0, s, c, slots, n, k_out, k_token_stride,
-                           k_head_stride, v_out, v_token_stride, v_head_stride, num_kv_heads, head_dim, page_size, sh);
-    else
-        hipLaunchKernelGGL((read_kernel<Bf16>), grid, dim3(256), 0, s, c, slots, n, k_out, k_token_stride,
-                           k_head_stride, v_out, v_token_stride, v_head_stride, num_kv_heads, head_dim, page_size, sh);
+    const int units = 2 * num_kv_heads * (head_dim / 8), several = units < 256 ? 256 / units : 1;
+    const dim3 grid((unsigned)((tokens + several - 1) / several), (unsigned)((units + 255) / 256 < 4 ? (units + 255) / 256 : 4));
+    const auto launch = [&](auto kernel) {
+        hipLaunchKernelGGL(kernel, grid, dim3(256), 0, (hipStream_t)stream, (const uint8_t *)cache, slots, tokens,
+                           num_pages * page_size, k_out, k_token_stride, k_head_stride, v_out, v_token_stride, v_head_stride,
+                           num_kv_heads, log2i(head_dim / 8), page_size, log2i(page_size), several);
+    };
+    if (element == kF32) launch(read_kernel<float>);
+    else if (element == kF16) launch(read_kernel<F16>);
+    else launch(read_kernel<Bf16>);
     return launch_status();
 }
