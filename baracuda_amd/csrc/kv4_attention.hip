@@ -870,7 +870,8 @@ int32_t sizes_ok(int num_seqs, int total_q, int max_q, int64_t max_kv, int hq, i
     if (!head_dim_ok(D) || !page_size_ok(ps) || element == kF32) return kUnsupported;
     if (num_pages > 0x7fffffff || max_kv > 0x7fffff00 || hq > 32768) return kUnsupported;
     const Cut c = cut_of(num_seqs, max_q, max_kv, hq / hk, hk, D, window);
-    if (c.grid > 0x7fffffff || c.items > 0x3fffffff || c.items * hk > 0x7fffffff) return kUnsupported;
+    // a launch has less than 2^32 threads, 512 of a workgroup at most
+    if (c.grid > 0x7fffff) return kUnsupported;
     return kOk;
 }
 

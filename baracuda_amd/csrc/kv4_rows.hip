@@ -332,7 +332,8 @@ int32_t sizes_ok(int64_t tokens, int hq, int hk, int D, int rope, int axes, int 
     if (tokens < 0 || hq < 0 || hk < 1 || D < 1 || rope < 0 || rope > D || axes < 1) return kInvalid;
     if (element < kF32 || element > kBf16) return kInvalid;
     if (D % 16 || D > 256 || rope % 16 || axes > 16) return kUnsupported;
-    if (tokens > 0x7fffffff || hq > 32768 || hk > 32768) return kUnsupported;
+    // a launch has less than 2^32 threads
+    if (tokens > 0x7fffff || hq > 32768 || hk > 32768) return kUnsupported;
     return kOk;
 }
 

@@ -297,7 +297,8 @@ extern "C" int32_t baracuda_kernels_kv_pages_fork_gfx950_run(int32_t layers, int
                                                              const int32_t *children, int32_t *fresh, void *stream) {
     const int32_t st = sizes_ok(layers, num_pages, page_bytes, page_size, rows, max_pages);
     if (st != kOk) return st;
-    if (count < 0 || count > 65536) return kInvalid;
+    if (count < 0) return kInvalid;
+    if (count > 65536) return kUnsupported;
     if (count == 0) return kOk;
     if (!cache || !tables || !lens || !refs || !parents || !children || !fresh) return kInvalid;
     const hipStream_t s = (hipStream_t)stream;
@@ -321,6 +322,7 @@ extern "C" int32_t baracuda_kernels_kv_pages_release_gfx950_run(int64_t num_page
     const int32_t st = sizes_ok(1, num_pages, 1, 1, rows, max_pages);
     if (st != kOk) return st;
     if (count < 0) return kInvalid;
+    if (count > 0x7fffff) return kUnsupported;    // a launch has less than 2^32 threads
     if (count == 0) return kOk;
     if (!tables || !lens || !refs || !which) return kInvalid;
     const unsigned y = (unsigned)((max_pages + 255) / 256);

@@ -210,6 +210,20 @@ def test_pages_operands():
     assert L.kv_pages_release_gfx950_run(5, 3, 6, 1, x, x, None, x, None) == 2
 
 
+def test_sizes_past_a_launch():
+    L, x = ffi.lib(), 4096
+    for tokens in (2 ** 23, 2 ** 31, 2 ** 60):
+        _raises(Unsupported, kv4.QkNormRopePlan.select, _qk(tokens=tokens))
+        _raises(Unsupported, kv4.Kv4AppendPlan.select, _append(tokens=tokens))
+        _raises(Unsupported, kv4.Kv4ReadPlan.select, kv4.Kv4ReadDescriptor(tokens, 2, 64, 16, 3))
+    _raises(Unsupported, kv4.Kv4AttentionPlan.select, _attn(num_seqs=2 ** 22, total_q=2 ** 22))
+    for name in ("num_heads", "head_dim", "page_size", "max_q", "max_pages"):       # past 32 bits, not cut off to them
+        _raises(Unsupported, kv4.Kv4AttentionPlan.select, _attn(**{name: 2 ** 32 + getattr(_attn(), name)}))
+    _raises(Unsupported, kv4.KvPagesPlan.select, kv4.KvPagesDescriptor(2, 5, 32, 4, 2 ** 32 + 3, 6))
+    assert L.kv_pages_release_gfx950_run(5, 3, 6, 2 ** 24, x, x, x, x, None) == 3
+    assert L.kv_pages_fork_gfx950_run(2, 5, 32, 4, 3, 6, 70000, x, x, x, x, x, x, x, None) == 3
+
+
 def test_plain_codec():
     """The oracle itself: borders, ties, the largest value of a scale, zeros, infinities."""
     x = torch.zeros(32, dtype=torch.float64)
