@@ -9,9 +9,9 @@
 // own running maximum and sum, and are joined through LDS at the end; parts of
 // a sequence that was cut are joined by a second kernel.
 //
-// Scores, maximum, sum and O are held in 32 bits.  P is rounded to the
-// element's type for the matrix product, at most half a step of a weight; the
-// sum is that of the weights before the rounding, whose mean error is none.
+// Scores, maximum, sum and O are held in 32 bits.  P is rounded to the element's
+// type for the matrix product, at most half a step of a weight, and the sum is that
+// of the rounded weights: what is divided by is what was multiplied with.
 #include "kv4_attention.hpp"
 
 namespace bk {
@@ -210,7 +210,7 @@ __global__ __launch_bounds__(64 * NW, OCC) void decode_kernel(const AttnArgs a) 
                 }
             }
             top = fmaxf(max_over_groups(top) * a.scale, m[mt]);
-            if (__any(top > m[mt] + kSlack)) {
+            if (__any(top > m[mt])) {
                 const float f = top > m[mt] ? exp2_fast(m[mt] - top) : 1.0f;
                 l[mt] *= f;
 #pragma unroll
@@ -226,8 +226,8 @@ __global__ __launch_bounds__(64 * NW, OCC) void decode_kernel(const AttnArgs a) 
                     e[j] = exp2_fast(__builtin_fmaf(sc[mt][n][j], a.scale, ref));
                     p[mt][n][0][j] = (int)pack2<T>(e[j], 0.0f);
                     p[mt][n][1][j] = (int)pack2<T>(0.0f, e[j]);
+                    l[mt] = add_pair<T>((uint32_t)p[mt][n][0][j], l[mt]);
                 }
-                l[mt] += (e[0] + e[1]) + (e[2] + e[3]);
             }
         }
         // O^T += V^T P^T.  A converted pair holds two values of one token, so the
