@@ -61,6 +61,14 @@ __device__ __forceinline__ int page_of(const AttnArgs &a, const int32_t *row, in
 
 // MT tiles of 16 rows; NT tiles of 16 tokens a step; NW waves; AHEAD: the next
 // step's loads go out before this one's products.
+//
+// Two tiles of tokens a step and three waves a SIMD: four tiles need a register
+// file that two waves fill (48 sequences 23.1 against 19.6 us, 200001 tokens of 8
+// heads 47.4 against 46.2), and four waves spill (70).  Two sequences of 200001 and
+// 15 tokens: 218 MB in 45.3 us (4.8 TB/s), 40.6 with the loads alone in the same
+// launch.  48 sequences of up to 8192: 47 MB in 16.8 us, of them 10 the loads' way
+// in and out.  One sequence of 777: 9.2 us, of them 8 a chain of loads (lengths,
+// table, page) on a cold cache.
 template <typename T, int D, int MT, int NT, int NW, int OCC, bool AHEAD = true>
 __global__ __launch_bounds__(64 * NW, OCC) void decode_kernel(const AttnArgs a) {
     constexpr int RB = 16 * MT, KW = D / 32, OC = D / 16;
@@ -393,6 +401,19 @@ __device__ __forceinline__ int item_in_line(const AttnArgs &a, int index) {
     return seq * a.row_blocks + block;
 }
 
+// Blocks of many rows: bound by issue, matrix and vector instructions in turn.
+//
+// S^T = K Q^T and O^T = V^T P^T as above, in 32x32x16 products, 32 rows a wave.
+// The waves convert a step's tokens together, each 16 of them, into LDS: K token
+// after token, V transposed, both in the order of the products' operands, so that
+// a row's weights stay where the scores were.  A conversion serves 256 rows (128
+// for heads of 256 values), where every wave of the small blocks converts for its
+// own 32: 38 M vector instructions against 66 M.  One buffer: a second one cost
+// as much in addresses as it saved (235 us each).  In the loop an
+// instruction of the matrix unit lies between some of the vector unit's; apart,
+// eight products and then 130 vector instructions, the two units took turns (252
+// against 235 us).  2047 tokens after 3953, with two shorter prompts, 32 heads of
+// 128 over 8: 169 GFLOP in 191 us, 886 TFLOP/s, a library's large product 1151.
 template <typename T, int D>
 __global__ __launch_bounds__(64 * prompt_waves(D), D == 256 ? 1 : 2) void prompt_kernel(const AttnArgs a) {
     constexpr int KS = D / 16, DB = D / 32, W = D / 32, NW = prompt_waves(D), TT = 16 * NW, ROWS = 32 * NW;
