@@ -413,7 +413,8 @@ __device__ __forceinline__ int item_in_line(const AttnArgs &a, int index) {
 // instruction of the matrix unit lies between some of the vector unit's; apart,
 // eight products and then 130 vector instructions, the two units took turns (252
 // against 235 us).  2047 tokens after 3953, with two shorter prompts, 32 heads of
-// 128 over 8: 169 GFLOP in 191 us, 886 TFLOP/s, a library's large product 1151.
+// 128 over 8: 169 GFLOP in 187 us, 902 TFLOP/s, a library's large product 1151; 2047
+// tokens alone, a triangle, 60 us (79 with blocks of neighbouring rows).
 template <typename T, int D>
 __global__ __launch_bounds__(64 * prompt_waves(D), D == 256 ? 1 : 2) void prompt_kernel(const AttnArgs a) {
     constexpr int KS = D / 16, DB = D / 32, W = D / 32, NW = prompt_waves(D), TT = 16 * NW, ROWS = 32 * NW;
@@ -428,6 +429,7 @@ __global__ __launch_bounds__(64 * prompt_waves(D), D == 256 ? 1 : 2) void prompt
 
     Part part;
     Item s;
+    int row0 = 32 * wave;          // the wave's first row, counted from s.first
     if (a.slots) {
         if (wave == 0) find_part(a, ROWS, index, lds_part, lds_item);
         __syncthreads();
@@ -438,20 +440,31 @@ __global__ __launch_bounds__(64 * prompt_waves(D), D == 256 ? 1 : 2) void prompt
         const int item = item_in_line(a, index);
         s = item_of(a, item, ROWS);
         if (s.rows <= 0) return;
+        if (a.paired) {
+            // half a block from the start and one from the end of the rows: every
+            // workgroup, and every SIMD (waves w and w + 4), has as much to do
+            constexpr int HALF = ROWS / 2;
+            const int all = s.n * a.ratio, blocks = (all + ROWS - 1) / ROWS, block = s.first / ROWS;
+            const int low = block * HALF, high = (2 * blocks - 1 - block) * HALF;
+            const int last = min(all, (high < all ? high : low) + HALF) - 1;
+            row0 = wave < NW / 2 ? low + 32 * wave : high + 32 * (wave - NW / 2);
+            s.first = 0, s.rows = all;
+            s.hi = max(0, min(s.len, s.base + token_of(a, last) + 1));
+        }
         part = Part{item, s.lo / 16, s.lo / 16 + tiles_of(s), 1, index};
     }
     s = uniform(s);
     part = uniform(part);
     const int t0 = part.t0, t1 = part.t1;
-    const int row = 32 * wave + n;
+    const int row = row0 + n;
     int lo, hi;
     row_span(a, s, row, lo, hi);
     // what all of the wave's rows see, and what any of them does
-    const int wave_rows = min(32, s.rows - 32 * wave);
+    const int wave_rows = min(32, s.rows - row0);
     int all_lo = 0, all_hi = 0, any_lo = 0, any_hi = 0;
     if (wave_rows > 0) {
-        row_span(a, s, 32 * wave + wave_rows - 1, all_lo, any_hi);
-        row_span(a, s, 32 * wave, any_lo, all_hi);
+        row_span(a, s, row0 + wave_rows - 1, all_lo, any_hi);
+        row_span(a, s, row0, any_lo, all_hi);
     }
     v4i q[KS];
 #pragma unroll
@@ -820,12 +833,12 @@ constexpr int whole_tokens(int D, int rows) { return rows > 16 || D == 256 ? 102
 // Blocks of 32 rows, whose waves share out the tokens, or of 256 (128 for heads of
 // 256 values), whose waves share the converted tokens?  The large blocks have a
 // longer way in and pay where there is work for all CUs: the measure is blocks of
-// 32 rows times tokens.  Large against small, us: heads of 128, 0.8 M 26 and 27,
-// 1.2 M 39 and 38, 2 M 38 and 43, 4.2 M 79 and 111, 24 M 240 and 278; below, 16
-// tokens of 8 heads before 4000 tokens (0.1 M) 23 and 13.  Heads of 256: 0.3 M 40
-// and 29, 0.6 M 47 and 64, 4.2 M 131 and 233.
+// 32 rows times tokens.  Large against small, us: heads of 128, 0.1 M 23 and 13, 0.6 M
+// 36 and 43 (one kv head), 0.8 M 34.5 and 35.4, 1.5 M 38 and 44, 4.2 M 60 and 111, 24 M
+// 187 and 278.  Heads of 64, 0.8 M 27 and 22, 1.2 M 32 and 28, 1.5 M 31 and 30, 4.2 M 45
+// and 80.  Heads of 256: 0.3 M 40 and 29, 0.6 M 47 and 64, 4.2 M 131 and 233.
 bool large_blocks(int64_t blocks, int64_t seen, int D) {
-    return blocks * seen >= (D == 256 ? 500000 : 1500000);
+    return blocks * seen >= (D == 64 ? 1500000 : D == 128 ? 700000 : 500000);
 }
 
 Cut cut_of(int num_seqs, int max_q, int64_t max_kv, int ratio, int hk, int D, int window) {
@@ -950,6 +963,7 @@ extern "C" int32_t baracuda_kernels_kv4_attention_gfx950_run(
     a.ratio_magic = a.ratio > 1 && rows * (uint64_t)a.ratio < (1ull << 32) ? (uint32_t)(((1ull << 32) + a.ratio - 1) / a.ratio) : 0;
     a.max_pages = max_pages, a.ps = page_size, a.ps_shift = log2i(page_size);
     a.causal = causal != 0, a.window = window;
+    a.paired = causal && !window && !c.slots && head_dim != 256;
     a.row_blocks = c.row_blocks, a.items = (int)c.items, a.slots = c.slots, a.min_tiles = c.min_tiles;
     a.scale = scale * 1.44269504088896340736f;
     const hipStream_t s = (hipStream_t)stream;

@@ -27,6 +27,7 @@ struct AttnArgs {
     int num_seqs, total_q, hq, hk, ratio, max_pages, ps, ps_shift, causal, window;
     int row_blocks;            // blocks of rows of a sequence
     int items;                 // num_seqs * row_blocks
+    int paired;                // large blocks take half their rows from a sequence's end
     int slots;                 // workgroups that the parts are made for; 0: nothing is split
     int min_tiles;             // tiles of 16 tokens that a part has at least
     float scale;               // times log2(e)
@@ -34,7 +35,7 @@ struct AttnArgs {
 
 // A block of rows and the tokens [lo, hi) that any of them sees.
 struct Item {
-    int seq, q0, first, rows, base, len, lo, hi;
+    int seq, q0, n, first, rows, base, len, lo, hi;
 };
 
 __device__ __forceinline__ int token_of(const AttnArgs &a, int row) {
@@ -54,6 +55,7 @@ __device__ __forceinline__ Item item_of(const AttnArgs &a, int item, int block) 
     const int len = a.lens[s.seq];
     const int64_t room = (int64_t)a.max_pages << a.ps_shift;
     s.q0 = q0;
+    s.n = n;
     s.base = len - n;
     s.len = (int)(len < room ? len : room);
     s.first = (item - s.seq * a.row_blocks) * block;
@@ -171,7 +173,7 @@ __device__ __forceinline__ void find_part(const AttnArgs &a, int block, int inde
 // The same in scalar registers: all lanes hold the same.
 __device__ __forceinline__ Item uniform(const Item &s) {
     const auto f = [](int x) { return __builtin_amdgcn_readfirstlane(x); };
-    return Item{f(s.seq), f(s.q0), f(s.first), f(s.rows), f(s.base), f(s.len), f(s.lo), f(s.hi)};
+    return Item{f(s.seq), f(s.q0), f(s.n), f(s.first), f(s.rows), f(s.base), f(s.len), f(s.lo), f(s.hi)};
 }
 __device__ __forceinline__ Part uniform(const Part &p) {
     const auto f = [](int x) { return __builtin_amdgcn_readfirstlane(x); };
