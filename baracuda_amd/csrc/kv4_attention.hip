@@ -838,7 +838,7 @@ constexpr int whole_tokens(int D, int rows) { return rows > 16 || D == 256 ? 102
 // 187 and 278.  Heads of 64, 0.8 M 27 and 22, 1.2 M 32 and 28, 1.5 M 31 and 30, 4.2 M 45
 // and 80.  Heads of 256: 0.3 M 40 and 29, 0.6 M 47 and 64, 4.2 M 131 and 233.
 bool large_blocks(int64_t blocks, int64_t seen, int D) {
-    return blocks * seen >= (D == 64 ? 1500000 : D == 128 ? 700000 : 500000);
+    return blocks * seen >= (D == 64 ? 1500000 : D == 128 ? 550000 : 500000);
 }
 
 Cut cut_of(int num_seqs, int max_q, int64_t max_kv, int ratio, int hk, int D, int window) {

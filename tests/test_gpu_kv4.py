@@ -455,6 +455,19 @@ def test_attention_in_large_blocks(gpu, case):
     _check_attention(got, q, cache, missing, lens_t, cu, causal, window, d ** -0.5)
 
 
+@pytest.mark.parametrize("d,ratio,dt", [(128, 8, BF), (64, 16, HF)], ids=str)
+@pytest.mark.parametrize("causal,window", [(True, 0), (True, 90), (False, 0)])
+def test_attention_in_blocks_from_both_ends(gpu, d, ratio, dt, causal, window):
+    """Prompts of several large blocks of rows that are not cut: a workgroup has rows from
+    the sequence's start and from its end, and an odd number of blocks a middle one."""
+    qs = [70, 33, 1, 0, 64, 2, 17, 1, 40, 3, 1]
+    lens = [70, 40, 300, 9, 64, 2, 200, 30, 41, 20, 1]
+    scene = _scene(torch.Generator().manual_seed(d), lens, qs, 8 * ratio, 8, d, 16, dt)
+    got = _attend(scene, 8, causal, window, max_kv=512)
+    cache, tables, lens_t, cu, q = scene
+    _check_attention(got, q, cache, tables, lens_t, cu, causal, window, d ** -0.5)
+
+
 @pytest.mark.parametrize("seqs", [40, 70])
 @pytest.mark.parametrize("most_q", [1, 41])
 @pytest.mark.parametrize("d,told", [(64, 900), (128, 3000), (256, 3000)])
