@@ -816,7 +816,6 @@ struct Cut {
     size_t part, bytes;
 };
 
-
 // Workgroups that the parts are made for: two a CU; heads of 256 values move
 // enough bytes with fewer (40 sequences of up to 6000 tokens: 384 25.5 us, 512 29.4).
 constexpr int slots_of(int D) { return D == 256 ? 384 : 512; }
@@ -959,7 +958,8 @@ extern "C" int32_t baracuda_kernels_kv4_attention_gfx950_run(
     a.num_seqs = num_seqs, a.total_q = total_q;
     a.hq = num_heads, a.hk = num_kv_heads, a.ratio = num_heads / num_kv_heads;
     // x magic / 2^32 falls short of the next whole number by less than x ratio / 2^32
-    const uint64_t rows = (uint64_t)max_q * (uint64_t)a.ratio + 512;
+    // (of any row there is, should a sequence have more tokens than max_q)
+    const uint64_t rows = (uint64_t)total_q * (uint64_t)a.ratio + 512;
     a.ratio_magic = a.ratio > 1 && rows * (uint64_t)a.ratio < (1ull << 32) ? (uint32_t)(((1ull << 32) + a.ratio - 1) / a.ratio) : 0;
     a.max_pages = max_pages, a.ps = page_size, a.ps_shift = log2i(page_size);
     a.causal = causal != 0, a.window = window;

@@ -122,14 +122,16 @@ struct Part {
 __device__ __forceinline__ void find_part(const AttnArgs &a, int block, int index, Part &part, Item &item) {
     const int lane = threadIdx.x & 63;
     Item s;
-    int total = 0;
+    // all tiles together may pass 32 bits: summed in two pieces
+    int high = 0, low = 0;
     for (int i0 = 0; i0 < a.items; i0 += 64) {
         s.rows = s.lo = s.hi = 0;
         if (i0 + lane < a.items) s = item_of(a, i0 + lane, block);
-        total += tiles_of(s);
+        high += tiles_of(s) >> 12, low += tiles_of(s) & 4095;
     }
-    total = __builtin_amdgcn_readlane(wave_scan(total), 63);
-    const int per = max(a.min_tiles, (int)(((int64_t)total * a.hk + a.slots - 1) / a.slots));
+    const int64_t total = ((int64_t)__builtin_amdgcn_readlane(wave_scan(high), 63) << 12) +
+                          __builtin_amdgcn_readlane(wave_scan(low), 63);
+    const int per = max(a.min_tiles, (int)((total * a.hk + a.slots - 1) / a.slots));
     int begin = 0;
     for (int i0 = 0; i0 < a.items; i0 += 64) {
         if (a.items > 64) {
