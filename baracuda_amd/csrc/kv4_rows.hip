@@ -199,7 +199,20 @@ __global__ __launch_bounds__(64 * kWaves) void rows_kernel(const RowArgs a, int 
                 float sum = 0;
 #pragma unroll
                 for (int i = 0; i < 8; ++i) sum = __builtin_fmaf(x[i], x[i], sum);
-                const float root = __builtin_amdgcn_rsqf(__builtin_fmaf(head_sum<float, G>(sum), a.inv_D, (float)a.eps));
+                const float mean = __builtin_fmaf(head_sum<float, G>(sum), a.inv_D, (float)a.eps);
+                float root = __builtin_amdgcn_rsqf(mean);
+                if constexpr (!__is_same(T, F16)) {
+                    // squares out of 32 bits' range, which f16's cannot be: the root of
+                    // the head times a power of two
+                    if (__any(!(mean > 0x1p-60f && mean < 0x1p126f))) {
+                        const float power = mean < 0x1p-60f ? 0x1p80f : mean < 0x1p126f ? 1.0f : 0x1p-80f;
+                        sum = 0;
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) sum = __builtin_fmaf(x[i] * power, x[i] * power, sum);
+                        sum = __builtin_fmaf(head_sum<float, G>(sum), a.inv_D, (float)(a.eps * power * power));
+                        root = power * __builtin_amdgcn_rsqf(sum);
+                    }
+                }
 #pragma unroll
                 for (int i = 0; i < 8; ++i) y[i] = root * __builtin_fmaf(z[i], sw[i], x[i] * cw[i]);
             } else {
@@ -217,13 +230,14 @@ __global__ __launch_bounds__(64 * kWaves) void rows_kernel(const RowArgs a, int 
                 if (norm) {
                     double sum = 0;
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) sum += (double)(x[i] * x[i]);   // 22 bits at most: exact
+                    for (int i = 0; i < 8; ++i) sum = __builtin_fma((double)x[i], (double)x[i], sum);
                     root = 1.0 / __builtin_sqrt(head_sum<double, G>(sum) / (double)a.D + a.eps);
                 }
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
                     float v = x[i], o = z[i];
-                    if (norm) v *= Raw<T>::get(mw, i), o *= Raw<T>::get(mz, inter ? i ^ 1 : i);   // exact as well
+                    // 22 bits at most: exact while it is in range
+                    if (norm) v *= Raw<T>::get(mw, i), o *= Raw<T>::get(mz, inter ? i ^ 1 : i);
                     const double t = turn ? __builtin_fma((double)v, (double)c[i], (double)o * (double)s[i]) : (double)v;
                     y[i] = Raw<T>::round((float)(t * root));
                 }

@@ -125,6 +125,53 @@ def test_qk_positions_out_of_range_give_nan(gpu):
         assert bad[1:3, :, :32].all() and not bad[1:3, :, 32:].any() and not bad[0].any() and not bad[3].any()
 
 
+@pytest.mark.parametrize("dt", [BF, FL], ids=str)
+@pytest.mark.parametrize("t", [5, 520])
+def test_qk_squares_out_of_range(gpu, dt, t):
+    # next to heads of ordinary size, heads whose squares 32 bits do not hold
+    d, eps = 128, 0.0
+    g = torch.Generator().manual_seed(6)
+    x = _rows(g, t, 4, d, FL)
+    x[:, 0] *= 1e25
+    x[:, 2] *= 1e-25
+    x[::2, 3] *= 2e35
+    x = x.to(dt)
+    w = (1 + 0.2 * torch.randn(d, generator=g)).to(dt)
+    rot = _rotation(g, t, 64, 1)
+    out = [torch.empty(t, 2, d, dtype=dt, device=gpu) for _ in range(2)]
+    kv4.QkNormRopePlan.select(kv4.QkNormRopeDescriptor(t, 2, 2, d, 64, KIND[dt], eps=eps)).run(
+        _dev(x[:, :2]), _dev(x[:, 2:]), *out, q_weight=_dev(w), k_weight=_dev(w), **_on_gpu(rot))
+    for got, part in ((out[0], x[:, :2]), (out[1], x[:, 2:])):
+        want, size = _plain_rows(part, w, eps, 64, rot, False)
+        _near(got, want, size, dt)
+
+
+@pytest.mark.parametrize("t", [5, 520])
+def test_append_squares_out_of_range(gpu, t):
+    hq, hk, d, ps = 1, 3, 64, 16
+    g = torch.Generator().manual_seed(7)
+    x = _rows(g, t, hq + 2 * hk, d, FL)
+    x[:, 0] *= 1e30
+    x[:, 1] *= 1e25
+    x[:, 2] *= 1e-25
+    x = x.to(BF)
+    w = (1 + 0.2 * torch.randn(d, generator=g)).to(BF)
+    rot = _rotation(g, t, d, 1)
+    pages = -(-t // ps)
+    cache = torch.zeros(pages, hk, kv4.head_bytes(ps, d), dtype=torch.uint8)
+    got, q_out = _dev(cache), torch.empty(t, hq, d, dtype=BF, device=gpu)
+    kv4.Kv4AppendPlan.select(kv4.Kv4AppendDescriptor(t, hq, hk, d, ps, pages, d, eps=0.0)).run(
+        _dev(x[:, hq:hq + hk]), _dev(x[:, hq + hk:]), got, _dev(torch.arange(t)), q=_dev(x[:, :hq]), q_out=q_out,
+        q_weight=_dev(w), k_weight=_dev(w), **_on_gpu(rot))
+    want, size = _plain_rows(x[:, :hq], w, 0.0, d, rot, False)
+    _near(q_out, want, size, BF)
+    k = _plain_rows(x[:, hq:hq + hk], w, 0.0, d, rot, False)[0].float().to(BF)
+    for i in range(t):
+        for h in range(hk):
+            plain.put(cache, i, h, k[i, h], x[i, hq + hk + h], plain.most(BF))
+    _same(got, cache, "cache")
+
+
 def test_qk_rows_of_zeros_and_infinities(gpu):
     t, d = 3, 128
     x = torch.zeros(t, 2, d, dtype=BF)
