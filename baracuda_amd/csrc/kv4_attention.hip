@@ -825,11 +825,10 @@ constexpr int kJoinWide = 2048;   // rows up to which four waves join one
 // Tokens up to which one workgroup of eight waves takes a sequence whole: parts
 // and their join cost a second launch.  One row, 8 kv heads, whole against cut,
 // us: heads of 128, 1100 tokens 10.0 and 12.0, 2000 14.9 and 12.1; of 64, 2000 12.5
-// and 12.3; of 256, 1100 12.8 and 12.6.  (Blocks of 32 rows have four waves: 1030
-// tokens 15.6 and 13.4.)
-constexpr int whole_tokens(int D, int rows) { return rows > 16 || D == 256 ? 1024 : D == 128 ? 1280 : 1792; }
+// and 12.3; of 256, 1100 12.8 and 12.6.  (Blocks of 32 rows see more and are cut.)
+constexpr int whole_tokens(int D) { return D == 256 ? 1024 : D == 128 ? 1280 : 1792; }
 
-// Blocks of 32 rows, whose waves share out the tokens, or of 256 (128 for heads of
+// Blocks of 16 or 32 rows, whose waves share out the tokens, or of 256 (128 for heads of
 // 256 values), whose waves share the converted tokens?  The large blocks have a
 // longer way in and pay where there is work for all CUs: the measure is blocks of
 // 32 rows times tokens.  Large against small, us: heads of 128, 0.1 M 23 and 13, 0.6 M
@@ -840,19 +839,29 @@ bool large_blocks(int64_t blocks, int64_t seen, int D) {
     return blocks * seen >= (D == 64 ? 1500000 : D == 128 ? 550000 : 500000);
 }
 
+// Blocks of 32 rows convert a token once for twice the rows of a block of 16, and
+// have fewer waves for it: they pay where the blocks fill the card and their
+// tokens are many.  16 rows against 32, us, heads of 64, 128, 256: 48 blocks of 32, 900
+// tokens 9.5, 11.0, 15.6 and 14.4, 17.6, 46.7; 1700 tokens 12.8, 14.3, 17.6 and 13.0,
+// 15.3, 26.6.  192 blocks, 6000 tokens 15.1, 23.4, 36.4 and 18.5, 23.3, 36.1.  320
+// blocks, 900 tokens 11.5, 13.8, 25.1 and 15.2, 18.5, 49.0; 1500 tokens 14.2, 21.6,
+// 29.9 and 14.2, 16.2, 27.0.
+constexpr int64_t kManyBlocks = 256, kManySeen = 1024;
+
 Cut cut_of(int num_seqs, int max_q, int64_t max_kv, int ratio, int hk, int D, int window) {
     Cut c{};
     const int64_t rows = (int64_t)max_q * ratio;
     const int64_t seen = window && window + (int64_t)max_q < max_kv ? window + (int64_t)max_q : max_kv;
-    const bool large = rows > 32 && large_blocks((rows + 31) / 32 * num_seqs * hk, seen, D);
-    c.rows = rows <= 16 ? 16 : large ? 32 * prompt_waves(D) : 32;
+    const int64_t blocks = (rows + 31) / 32 * num_seqs * hk;
+    const bool large = rows > 32 && large_blocks(blocks, seen, D);
+    c.rows = large ? 32 * prompt_waves(D) : rows > 16 && blocks >= kManyBlocks && seen > kManySeen ? 32 : 16;
     c.row_blocks = (int)((rows + c.rows - 1) / c.rows);
     c.items = (int64_t)num_seqs * c.row_blocks;
     if (large) {
         c.slots = seen <= 512 || c.items * hk >= 256 ? 0 : 256;
         c.min_tiles = 2 * kMinTiles;
     } else {
-        c.slots = seen <= whole_tokens(D, c.rows) || c.items * hk >= 4096 ? 0 : slots_of(D);
+        c.slots = (c.rows == 16 && seen <= whole_tokens(D)) || c.items * hk >= 4096 ? 0 : slots_of(D);
         c.min_tiles = kMinTiles;
     }
     c.wide = !c.slots && c.rows == 16 && seen > 256 && c.items * hk <= 256;

@@ -533,6 +533,27 @@ def test_attention_many_sequences(gpu, seqs, most_q, d, told):
     _check_attention(got, q, cache, tables, lens_t, cu, True, 0, d ** -0.5)
 
 
+@pytest.mark.parametrize("d,dt", [(64, HF), (128, BF), (256, BF)], ids=str)
+@pytest.mark.parametrize("causal,window", [(True, 0), (True, 90), (False, 0)])
+def test_attention_in_blocks_of_32(gpu, d, dt, causal, window):
+    """Blocks of 32 rows, one and two a sequence, enough of them to fill the card, some cut."""
+    rng = random.Random(d)
+    qs = [rng.randint(0, 12) for _ in range(35)]
+    lens = [q + rng.randint(0, 40) for q in qs]
+    qs[0], lens[0], qs[9], lens[9], qs[20], lens[20] = 11, 64, 12, 1400, 1, 333
+    scene = _scene(torch.Generator().manual_seed(d), lens, qs, 24, 8, d, 16, dt)
+    cache, tables, lens_t, cu, q = scene
+    got = _attend(scene, 8, causal, window, max_kv=1500).cpu()
+    _check_attention(got, q, cache, tables, lens_t, cu, causal, window, d ** -0.5)
+    if causal:      # a NaN in V of token 61 of 64: rows 8 to 10 of the first sequence see it
+        cache[int(tables[0, 3]), :, plain.places(16, d)[3][13, 1]] = 255
+        odd = _attend((cache, tables, lens_t, cu, q), 8, causal, window, max_kv=1500).cpu()
+        assert torch.isnan(odd[8:11, :, 32:64]).all()
+        rest = torch.ones_like(odd, dtype=torch.bool)
+        rest[8:11, :, 32:64] = False
+        assert not torch.isnan(odd[rest]).any() and torch.equal(odd[11:], got[11:])
+
+
 # ---- pages -----------------------------------------------------------------------
 def _pages_plan(layers, pages, size, ps, rows, width):
     return kv4.KvPagesPlan.select(kv4.KvPagesDescriptor(layers, pages, size, ps, rows, width))
