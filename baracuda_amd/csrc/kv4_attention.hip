@@ -828,17 +828,6 @@ constexpr int kJoinWide = 2048;   // rows up to which four waves join one
 // and 12.3; of 256, 1100 12.8 and 12.6.  (Blocks of 32 rows see more and are cut.)
 constexpr int whole_tokens(int D) { return D == 256 ? 1024 : D == 128 ? 1280 : 1792; }
 
-// Blocks of 16 or 32 rows, whose waves share out the tokens, or of 256 (128 for heads of
-// 256 values), whose waves share the converted tokens?  The large blocks have a
-// longer way in and pay where there is work for all CUs: the measure is blocks of
-// 32 rows times tokens.  Large against small, us: heads of 128, 0.1 M 23 and 13, 0.6 M
-// 36 and 43 (one kv head), 0.8 M 34.5 and 35.4, 1.5 M 38 and 44, 4.2 M 60 and 111, 24 M
-// 187 and 278.  Heads of 64, 0.8 M 27 and 22, 1.2 M 32 and 28, 1.5 M 31 and 30, 4.2 M 45
-// and 80.  Heads of 256: 0.3 M 40 and 29, 0.6 M 47 and 64, 4.2 M 131 and 233.
-bool large_blocks(int64_t blocks, int64_t seen, int D) {
-    return blocks * seen >= (D == 64 ? 1500000 : D == 128 ? 550000 : 500000);
-}
-
 // Blocks of 32 rows convert a token once for twice the rows of a block of 16, and
 // have fewer waves for it: they pay where the blocks fill the card and their
 // tokens are many.  16 rows against 32, us, heads of 64, 128, 256: 48 blocks of 32, 900
@@ -847,6 +836,20 @@ bool large_blocks(int64_t blocks, int64_t seen, int D) {
 // blocks, 900 tokens 11.5, 13.8, 25.1 and 15.2, 18.5, 49.0; 1500 tokens 14.2, 21.6,
 // 29.9 and 14.2, 16.2, 27.0.
 constexpr int64_t kManyBlocks = 256, kManySeen = 1024;
+
+// Blocks of 16 or 32 rows, whose waves share out the tokens, or of 256 (128 for heads of
+// 256 values), whose waves share the converted tokens?  The large blocks have a
+// longer way in and pay where there is work for all CUs: the measure is blocks of
+// 32 rows times tokens.  Large against small, us: heads of 128, 0.1 M 23 and 13, 0.6 M
+// 36 and 43 (one kv head), 0.8 M 34.5 and 35.4, 1.5 M 38 and 44, 4.2 M 60 and 111, 24 M
+// 187 and 278.  Heads of 64, 0.8 M 27 and 22, 1.2 M 32 and 28, 1.5 M 31 and 30, 4.2 M 45
+// and 80.  Heads of 256: 0.3 M 40 and 29, 0.6 M 47 and 64, 4.2 M 131 and 233.  Up to
+// kManySeen tokens against blocks of 16: heads of 128, 0.8 M 39 and 25, 2 M 36 and 36
+// (of 500 tokens 35 and 44); of 256, 0.8 M 50 and 42, 2 M 59 and 71.
+bool large_blocks(int64_t blocks, int64_t seen, int D) {
+    if (seen <= kManySeen) return blocks * seen >= (D == 256 ? 1200000 : 1500000);
+    return blocks * seen >= (D == 64 ? 1500000 : D == 128 ? 550000 : 500000);
+}
 
 Cut cut_of(int num_seqs, int max_q, int64_t max_kv, int ratio, int hk, int D, int window) {
     Cut c{};

@@ -533,6 +533,16 @@ def test_attention_many_sequences(gpu, seqs, most_q, d, told):
     _check_attention(got, q, cache, tables, lens_t, cu, True, 0, d ** -0.5)
 
 
+@pytest.mark.parametrize("causal,window", [(True, 0), (True, 90), (False, 0)])
+def test_attention_in_blocks_from_both_ends_told_of_1024_tokens(gpu, causal, window):
+    qs = [70, 33, 1, 0, 64, 2, 17, 1, 40, 3, 1]
+    lens = [70, 40, 300, 9, 64, 2, 200, 30, 41, 20, 1]
+    scene = _scene(torch.Generator().manual_seed(3), lens, qs, 64, 8, 128, 16, BF)
+    got = _attend(scene, 8, causal, window, max_kv=1024)
+    cache, tables, lens_t, cu, q = scene
+    _check_attention(got, q, cache, tables, lens_t, cu, causal, window, 128 ** -0.5)
+
+
 @pytest.mark.parametrize("d,dt", [(64, HF), (128, BF), (256, BF)], ids=str)
 @pytest.mark.parametrize("causal,window", [(True, 0), (True, 90), (False, 0)])
 def test_attention_in_blocks_of_32(gpu, d, dt, causal, window):
