@@ -442,9 +442,11 @@ __global__ __launch_bounds__(64 * prompt_waves(D), D == 256 ? 1 : 2) void prompt
         if (s.rows <= 0) return;
         if (a.paired) {
             // half a block from the start and one from the end of the rows: every
-            // workgroup, and every SIMD (waves w and w + 4), has as much to do
+            // workgroup, and every SIMD (waves w and w + 4), has as much to do.  The rows
+            // end with the launch's blocks, also of a sequence that has more of them.
             constexpr int HALF = ROWS / 2;
-            const int all = s.n * a.ratio, blocks = (all + ROWS - 1) / ROWS, block = s.first / ROWS;
+            const int all = min(s.n * a.ratio, a.row_blocks * ROWS);
+            const int blocks = (all + ROWS - 1) / ROWS, block = s.first / ROWS;
             const int low = block * HALF, high = (2 * blocks - 1 - block) * HALF;
             const int last = min(all, (high < all ? high : low) + HALF) - 1;
             row0 = wave < NW / 2 ? low + 32 * wave : high + 32 * (wave - NW / 2);
