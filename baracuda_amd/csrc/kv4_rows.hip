@@ -20,7 +20,8 @@
 // factors multiplied once 36; six rounds 33.5 (twelve 33.8).  8191 tokens of 16 + 4
 // heads of 256 into the cache: 156 MB in 46 us.
 //
-// Q, and K without a cache, are computed in 32 bits and rounded once.  K that
+// Q, and K without a cache, are computed in 32 bits and rounded once (heads that
+// leave their range, in 64).  K that
 // is quantized is computed in 64 bits: it is rounded to the element's type
 // first and then to 4 bits, and a value next to a border between two codes has
 // to fall on the side of the exact one, or equal prefixes would give unequal
@@ -160,13 +161,52 @@ __global__ __launch_bounds__(64 * kWaves) void rows_kernel(const RowArgs a, int 
     Mem mw{}, mz{};
     float cw[8], sw[8];
     int held = -1;
+    uint32_t redo = 0;             // rounds that 32 bits do not hold
+
+    const auto top_of = [](const float (&y)[8]) {
+        uint32_t top = 0;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(y[i]) & 0x7fffffffu);
+        return top;
+    };
+    // K's or V's codes, and the scale that four lanes share; top: the lane's own top_of
+    const auto store_codes = [&](int kind, int head, const float (&y)[8], uint32_t top) {
+        top = max(top, across<1>(top));
+        top = max(top, across<2>(top));
+        const bool good = top < 0x7f800000u;
+        const int byte = good ? scale_byte(top, a.most) : 255;
+        const uint32_t code = good ? encode8(y, byte) : 0u;
+        if (at >= a.D || head >= a.hk || slot < 0 || slot >= a.num_slots) return;
+        const int off = (int)(slot & (a.ps - 1)), few = a.D / 32;
+        uint8_t *base = a.cache + ((slot >> a.ps_shift) * a.hk + head) * head_bytes(a.ps, a.D);
+        if (kind == 1) {
+            *(uint32_t *)(base + off * (a.D / 2) + 4 * l) = code;
+            if (l % 4 == 0) base[k_scales(a.ps, a.D) + off * few + l / 4] = (uint8_t)byte;
+        } else {
+            uint8_t *p = base + v_codes(a.ps, a.D) + (off >> 2) * 64 * few + (off & 3) * few;
+            if (few == 2) {          // a lane holds two runs
+                *(uint16_t *)(p + (2 * l) * 8) = (uint16_t)code;
+                *(uint16_t *)(p + (2 * l + 1) * 8) = (uint16_t)(code >> 16);
+            } else if (few == 4) {   // one
+                *(uint32_t *)(p + l * 16) = code;
+            } else {                 // or half of one
+                *(uint32_t *)(p + (l / 2) * 32 + (l & 1) * 4) = code;
+            }
+            if (l % 4 == 0) base[v_scales(a.ps, a.D) + ((off >> 2) * few + l / 4) * 4 + (off & 3)] = (uint8_t)byte;
+        }
+    };
+    const auto store_row = [&](int kind, int head, const float (&y)[8]) {
+        if (at >= a.D || head >= (kind ? a.hk : a.hq)) return;
+        Mem out;
+        Raw<T>::put(out, y);
+        *(Mem *)((char *)a.dst[kind] + (token * a.dst_token[kind] + head * a.dst_head[kind] + at) * SIZE) = out;
+    };
 
 #pragma unroll
     for (int it = 0; it < ITERS; ++it) {
         const int r = first + it;
         if (r >= rounds) break;
         const int kind = kind_of(r), head = head_of(r, kind);
-        const bool mine = at < a.D && head < (kind ? a.hk : a.hq);
         if (norm && kind < 2 && kind != held) {
             held = kind;
             if (at < a.D) {
@@ -200,39 +240,35 @@ __global__ __launch_bounds__(64 * kWaves) void rows_kernel(const RowArgs a, int 
 #pragma unroll
                 for (int i = 0; i < 8; ++i) sum = __builtin_fmaf(x[i], x[i], sum);
                 const float mean = __builtin_fmaf(head_sum<float, G>(sum), a.inv_D, (float)a.eps);
-                float root = __builtin_amdgcn_rsqf(mean);
-                if constexpr (!__is_same(T, F16)) {
-                    // squares out of 32 bits' range, which f16's cannot be: the root of
-                    // the head times a power of two
-                    if (__any(!(mean > 0x1p-60f && mean < 0x1p126f))) {
-                        const float power = mean < 0x1p-60f ? 0x1p80f : mean < 0x1p126f ? 1.0f : 0x1p-80f;
-                        sum = 0;
-#pragma unroll
-                        for (int i = 0; i < 8; ++i) sum = __builtin_fmaf(x[i] * power, x[i] * power, sum);
-                        sum = __builtin_fmaf(head_sum<float, G>(sum), a.inv_D, (float)(a.eps * power * power));
-                        root = power * __builtin_amdgcn_rsqf(sum);
-                    }
-                }
+                const float root = __builtin_amdgcn_rsqf(mean);
 #pragma unroll
                 for (int i = 0; i < 8; ++i) y[i] = root * __builtin_fmaf(z[i], sw[i], x[i] * cw[i]);
+                if constexpr (!__is_same(T, F16)) {
+                    // of a pair's two products that leave the range, one sum at least is infinite
+                    float high = 0.0f;
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) high = fmaxf(high, __builtin_fabsf(y[i]));
+                    if (__any(!(mean > 0x1p-40f && mean < 0x1p100f && high < INFINITY))) {
+                        redo |= 1u << it;
+                        continue;
+                    }
+                }
             } else {
 #pragma unroll
                 for (int i = 0; i < 8; ++i) y[i] = turn ? __builtin_fmaf(z[i], s[i], x[i] * c[i]) : x[i];
             }
-            if (mine) {
-                Mem out;
-                Raw<T>::put(out, y);
-                *(Mem *)((char *)a.dst[kind] + (token * a.dst_token[kind] + head * a.dst_head[kind] + at) * SIZE) = out;
-            }
+            store_row(kind, head, y);
         } else if constexpr (KV4) {
+            uint32_t top;
             if (kind == 1) {
-                double root = 1;
+                double root = 1, sum = 0;
                 if (norm) {
-                    double sum = 0;
 #pragma unroll
                     for (int i = 0; i < 8; ++i) sum = __builtin_fma((double)x[i], (double)x[i], sum);
-                    root = 1.0 / __builtin_sqrt(head_sum<double, G>(sum) / (double)a.D + a.eps);
+                    sum = head_sum<double, G>(sum);
+                    root = 1.0 / __builtin_sqrt(sum / (double)a.D + a.eps);
                 }
+                float least = INFINITY;
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
                     float v = x[i], o = z[i];
@@ -240,39 +276,62 @@ __global__ __launch_bounds__(64 * kWaves) void rows_kernel(const RowArgs a, int 
                     if (norm) v *= Raw<T>::get(mw, i), o *= Raw<T>::get(mz, inter ? i ^ 1 : i);
                     const double t = turn ? __builtin_fma((double)v, (double)c[i], (double)o * (double)s[i]) : (double)v;
                     y[i] = Raw<T>::round((float)(t * root));
+                    least = fminf(least, __builtin_fabsf(y[i]));
+                }
+                top = top_of(y);
+                if constexpr (!__is_same(T, F16)) {
+                    // a product past the range, or bits of one below it
+                    if (norm && __any(sum != 0 && !(least >= 0x1p-60f && top < 0x7f800000u && root < 0x1p30))) {
+                        redo |= 1u << it;
+                        continue;
+                    }
                 }
             } else {
 #pragma unroll
                 for (int i = 0; i < 8; ++i) y[i] = x[i];
+                top = top_of(y);
             }
-            // four lanes share a scale
-            uint32_t top = 0;
+            store_codes(kind, head, y, top);
+        }
+    }
+
+    // Heads whose squares or products with the weights leave 32 bits (f16's cannot): from
+    // the inputs on in 64, a round at a time
+    if constexpr (!__is_same(T, F16)) {
+        for (; redo; redo &= redo - 1) {
+            // a copy of its own: addresses kept from above cost the loop above a register (97,
+            // a wave a SIMD less)
+            int place = at;
+            asm volatile("" : "+v"(place));
+            const int r = first + __builtin_ctz(redo), kind = kind_of(r), head = head_of(r, kind);
+            Mem m{}, w{}, u{}, far;
+            if (at < a.D) {
+                if (head < (kind ? a.hk : a.hq))
+                    m = *(const Mem *)((const char *)a.src[kind] + (token * a.src_token[kind] + head * a.src_head[kind] + at) * SIZE);
+                w = *(const Mem *)((const char *)a.weight[kind] + at * SIZE);
+                u = *(const Mem *)((const char *)a.weight[kind] + 8 * other * SIZE);
+            }
 #pragma unroll
-            for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(y[i]) & 0x7fffffffu);
-            top = max(top, across<1>(top));
-            top = max(top, across<2>(top));
-            const bool good = top < 0x7f800000u;
-            const int byte = good ? scale_byte(top, a.most) : 255;
-            const uint32_t code = good ? encode8(y, byte) : 0u;
-            if (mine && slot >= 0 && slot < a.num_slots) {
-                const int off = (int)(slot & (a.ps - 1)), few = a.D / 32;
-                uint8_t *base = a.cache + ((slot >> a.ps_shift) * a.hk + head) * head_bytes(a.ps, a.D);
-                if (kind == 1) {
-                    *(uint32_t *)(base + off * (a.D / 2) + 4 * l) = code;
-                    if (l % 4 == 0) base[k_scales(a.ps, a.D) + off * few + l / 4] = (uint8_t)byte;
-                } else {
-                    uint8_t *p = base + v_codes(a.ps, a.D) + (off >> 2) * 64 * few + (off & 3) * few;
-                    if (few == 2) {          // a lane holds two runs
-                        *(uint16_t *)(p + (2 * l) * 8) = (uint16_t)code;
-                        *(uint16_t *)(p + (2 * l + 1) * 8) = (uint16_t)(code >> 16);
-                    } else if (few == 4) {   // one
-                        *(uint32_t *)(p + l * 16) = code;
-                    } else {                 // or half of one
-                        *(uint32_t *)(p + (l / 2) * 32 + (l & 1) * 4) = code;
-                    }
-                    if (l % 4 == 0) base[v_scales(a.ps, a.D) + ((off >> 2) * few + l / 4) * 4 + (off & 3)] = (uint8_t)byte;
+            for (int i = 0; i < W; ++i) far.w[i] = (uint32_t)__shfl((int)m.w[i], other, G);
+            double sum = 0;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) sum = __builtin_fma((double)Raw<T>::get(m, i), (double)Raw<T>::get(m, i), sum);
+            const double root = 1.0 / __builtin_sqrt(head_sum<double, G>(sum) / (double)a.D + a.eps);
+            float y[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const double v = (double)Raw<T>::get(m, i) * (double)Raw<T>::get(w, i);
+                const double o = (double)Raw<T>::get(far, inter ? i ^ 1 : i) * (double)Raw<T>::get(u, inter ? i ^ 1 : i);
+                double t = v;
+                if (turn) {
+                    const int p = inter ? place / 2 + i / 2 : (low ? place : place - half) + i;
+                    const double cosine = lc[p], sine = (inter ? (i & 1) == 0 : low) ? -ls[p] : ls[p];
+                    t = __builtin_fma(v, cosine, o * sine);
                 }
+                y[i] = Raw<T>::round((float)(t * root));
             }
+            if (KV4 && kind) store_codes(kind, head, y, top_of(y));
+            else store_row(kind, head, y);
         }
     }
 }

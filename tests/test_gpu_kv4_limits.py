@@ -5,7 +5,8 @@ import torch
 from baracuda_amd import kv4
 from tests import kv4_plain as plain
 from tests.gpu_util import sync
-from tests.test_gpu_kv4 import BF, KIND, _check_attention, _dev, _scene
+from tests.test_gpu_kv4 import (BF, FL, KIND, _check_attention, _dev, _near, _on_gpu, _plain_rows, _rotation, _rows, _same,
+                                _scene)
 
 pytestmark = pytest.mark.gpu
 
@@ -48,3 +49,78 @@ def test_attention_of_a_sequence_longer_than_max_q(gpu, case):
     # the rows past max_q are not the call's: take them out of the comparison
     got[past] = want[past].to(BF)
     _check_attention(got, q, cache, tables, lens_t, cu, causal, window, d ** -0.5)
+
+
+# ---- heads and weights at the ends of the range -------------------------------
+@pytest.mark.parametrize("inter", [False, True])
+@pytest.mark.parametrize("dt", [BF, FL], ids=str)
+@pytest.mark.parametrize("t", [5, 520])
+def test_qk_products_out_of_range(gpu, dt, t, inter):
+    # values and their products with the weights past the largest number, where the
+    # normed values are of ordinary size, and heads of the smallest numbers there are
+    d, rope = 128, 64
+    g = torch.Generator().manual_seed(16)
+    x = _rows(g, t, 6, d, FL)
+    x[:, 0] = x[:, 0].sign() * 3e38 * (0.5 + 0.5 * torch.rand(t, d, generator=g))
+    x[:, 1, ::7] = 3.3e38
+    x[:, 3] = x[:, 3].sign() * torch.finfo(dt).max
+    x[:, 4] = x[:, 4].sign() * (torch.finfo(dt).tiny * torch.finfo(dt).eps) * torch.randint(1, 9, (t, d), generator=g)
+    x[:, 5] *= 1e-30
+    x = x.to(dt)
+    assert torch.isfinite(x).all()
+    w = (1.3 + 0.2 * torch.randn(d, generator=g)).to(dt)
+    rot = _rotation(g, t, rope, 1)
+    out = [torch.empty(t, 3, d, dtype=dt, device=gpu) for _ in range(2)]
+    kv4.QkNormRopePlan.select(kv4.QkNormRopeDescriptor(t, 3, 3, d, rope, KIND[dt], interleaved=inter, eps=0.0)).run(
+        _dev(x[:, :3]), _dev(x[:, 3:]), *out, q_weight=_dev(w), k_weight=_dev(w), **_on_gpu(rot))
+    for got, part in ((out[0], x[:, :3]), (out[1], x[:, 3:])):
+        want, size = _plain_rows(part, w, 0.0, rope, rot, inter)
+        _near(got, want, size, dt)
+
+
+@pytest.mark.parametrize("t", [5, 520])
+def test_qk_weights_out_of_range(gpu, t):
+    # ordinary heads under large weights, and large ones under those
+    d, eps = 128, 1e-6
+    g = torch.Generator().manual_seed(17)
+    x = _rows(g, t, 2, d, FL)
+    x[:, 1] *= 1e16
+    x = x.to(BF)
+    w = ((1 + 0.2 * torch.randn(d, generator=g)) * 1e25).to(BF)
+    rot = _rotation(g, t, 64, 1)
+    out = [torch.empty(t, 1, d, dtype=BF, device=gpu) for _ in range(2)]
+    kv4.QkNormRopePlan.select(kv4.QkNormRopeDescriptor(t, 1, 1, d, 64, eps=eps)).run(
+        _dev(x[:, :1]), _dev(x[:, 1:]), *out, q_weight=_dev(w), k_weight=_dev(w), **_on_gpu(rot))
+    for got, part in ((out[0], x[:, :1]), (out[1], x[:, 1:])):
+        want, size = _plain_rows(part, w, eps, 64, rot, False)
+        _near(got, want, size, BF)
+
+
+@pytest.mark.parametrize("d,rope,inter", [(64, 64, False), (128, 64, True), (256, 0, False)])
+@pytest.mark.parametrize("t", [5, 520])
+def test_append_products_out_of_range(gpu, t, d, rope, inter):
+    hq, hk, ps = 1, 4, 16
+    g = torch.Generator().manual_seed(18)
+    x = _rows(g, t, hq + 2 * hk, d, FL)
+    x[:, 0] = x[:, 0].sign() * 3e38
+    x[:, 1] = x[:, 1].sign() * 3e38 * (0.3 + 0.7 * torch.rand(t, d, generator=g))
+    x[:, 2, ::5] = 3.3e38
+    x[:, 3] *= 1e-37
+    x[:, 4] = x[:, 4].sign() * 2.0 ** -133 * torch.randint(1, 9, (t, d), generator=g)
+    x = x.to(BF)
+    assert torch.isfinite(x).all()
+    w = (1.3 + 0.2 * torch.randn(d, generator=g)).to(BF)
+    rot = _rotation(g, t, rope, 1)
+    pages = -(-t // ps)
+    cache = torch.zeros(pages, hk, kv4.head_bytes(ps, d), dtype=torch.uint8)
+    got, q_out = _dev(cache), torch.empty(t, hq, d, dtype=BF, device=gpu)
+    kv4.Kv4AppendPlan.select(kv4.Kv4AppendDescriptor(t, hq, hk, d, ps, pages, rope, interleaved=inter, eps=0.0)).run(
+        _dev(x[:, hq:hq + hk]), _dev(x[:, hq + hk:]), got, _dev(torch.arange(t)), q=_dev(x[:, :hq]), q_out=q_out,
+        q_weight=_dev(w), k_weight=_dev(w), **_on_gpu(rot))
+    want, size = _plain_rows(x[:, :hq], w, 0.0, rope, rot, inter)
+    _near(q_out, want, size, BF)
+    k = _plain_rows(x[:, hq:hq + hk], w, 0.0, rope, rot, inter)[0].float().to(BF)
+    for i in range(t):
+        for h in range(hk):
+            plain.put(cache, i, h, k[i, h], x[i, hq + hk + h], plain.most(BF))
+    _same(got, cache, "cache")
