@@ -43,6 +43,13 @@ __device__ __forceinline__ int token_of(const AttnArgs &a, int row) {
     return a.ratio_magic ? (int)__umulhi((uint32_t)row, a.ratio_magic) : row / a.ratio;
 }
 
+// The first position that the window of a row at `pos` holds.  A row before the cache's
+// start (more new tokens than it holds) has a negative one: no difference of the
+// two, which may pass 32 bits.
+__device__ __forceinline__ int first_seen(const AttnArgs &a, int pos) {
+    return a.window && pos >= a.window ? pos - a.window + 1 : 0;
+}
+
 __device__ __forceinline__ Item item_of(const AttnArgs &a, int item, int block) {
     Item s;
     s.seq = a.row_blocks == 1 ? item : item / a.row_blocks;
@@ -64,7 +71,7 @@ __device__ __forceinline__ Item item_of(const AttnArgs &a, int item, int block) 
     if (s.rows > 0) {
         const int i0 = token_of(a, s.first), i1 = token_of(a, s.first + s.rows - 1);
         s.hi = max(0, a.causal ? min(s.len, s.base + i1 + 1) : s.len);
-        s.lo = a.window ? max(0, s.base + i0 - a.window + 1) : 0;
+        s.lo = first_seen(a, s.base + i0);
     }
     return s;
 }
@@ -76,7 +83,7 @@ __device__ __forceinline__ void row_span(const AttnArgs &a, const Item &s, int r
     const int pos = s.base + token_of(a, s.first + r);
     const bool in = r < s.rows;
     hi = in ? (a.causal ? min(s.len, pos + 1) : s.len) : 0;
-    lo = in && a.window ? max(0, pos - a.window + 1) : 0;
+    lo = in ? first_seen(a, pos) : 0;
 }
 
 __device__ __forceinline__ float as_float(uint32_t x) { return __uint_as_float(x); }

@@ -124,3 +124,20 @@ def test_append_products_out_of_range(gpu, t, d, rope, inter):
         for h in range(hk):
             plain.put(cache, i, h, k[i, h], x[i, hq + hk + h], plain.most(BF))
     _same(got, cache, "cache")
+
+
+# ---- windows --------------------------------------------------------------------
+WINDOWS = [([40], [64], 4, 2, 64, 200), ([40], [64], 4, 2, 64, 2_000_000), ([3, 0, 30], [9, 5, 30], 16, 2, 128, 900),
+           ([600, 5], [257, 129], 8, 2, 256, 2_000_000)]
+
+
+@pytest.mark.parametrize("window", [2 ** 31 - 1, 2 ** 31 - 60])
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("case", WINDOWS, ids=str)
+def test_attention_windows_that_hide_nothing(gpu, case, causal, window):
+    """The widest windows, also with more new tokens than the cache holds."""
+    lens, qs, hq, hk, d, max_kv = case
+    scene = _scene(torch.Generator().manual_seed(sum(qs)), lens, qs, hq, hk, d, 16, BF)
+    cache, tables, lens_t, cu, q = scene
+    got = _attend(scene, hk, max(qs), max_kv, causal, window)
+    _check_attention(got, q, cache, tables, lens_t, cu, causal, 0, d ** -0.5)
