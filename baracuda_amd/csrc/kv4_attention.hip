@@ -126,6 +126,7 @@ __global__ __launch_bounds__(64 * NW, OCC) void decode_kernel(const AttnArgs a) 
     const int32_t *table = a.tables + s.seq * a.table_stride;
     v4f o[MT][OC];
     float m[MT], l[MT];
+    const float room = headroom<T>(s.len, 0.0f);
     uint32_t poison[MT];           // of a row, the lane's runs that a NaN has reached
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt) {
@@ -217,7 +218,7 @@ __global__ __launch_bounds__(64 * NW, OCC) void decode_kernel(const AttnArgs a) 
                     top = fmaxf(top, sc[mt][n][j]);
                 }
             }
-            top = fmaxf(max_over_groups(top) * a.scale, m[mt]);
+            top = fmaxf(__builtin_fmaf(max_over_groups(top), a.scale, room), m[mt]);
             if (__any(top > m[mt])) {
                 const float f = top > m[mt] ? exp2_fast(m[mt] - top) : 1.0f;
                 l[mt] *= f;
@@ -581,6 +582,7 @@ __global__ __launch_bounds__(64 * prompt_waves(D), D == 256 ? 1 : 2) void prompt
 #pragma unroll
         for (int i = 0; i < 16; ++i) o[d][i] = 0.0f;
     float m = -INFINITY, l = 0.0f;
+    const float room = headroom<T>(s.len, kSlack);
     uint32_t poison = 0;           // blocks of 32 values that a NaN has reached
 
     const auto products = [&](int t, uint32_t there) {
@@ -618,7 +620,7 @@ __global__ __launch_bounds__(64 * prompt_waves(D), D == 256 ? 1 : 2) void prompt
         for (int b = 0; b < NW / 2; ++b) {
             const bool last = b + 1 == NW / 2;
             const auto both = __builtin_amdgcn_permlane32_swap(__float_as_uint(top), __float_as_uint(top), false, false);
-            top = fmaxf(fmaxf(as_float(both[0]), as_float(both[1])) * a.scale, m);
+            top = fmaxf(__builtin_fmaf(fmaxf(as_float(both[0]), as_float(both[1])), a.scale, room), m);
             if (__any(top > m + kSlack)) {
                 const float f = top > m ? exp2_fast(m - top) : 1.0f;
                 l *= f;

@@ -247,10 +247,20 @@ __device__ __forceinline__ float add_pair(uint32_t pair, float l) {
 
 // How far (in powers of two) a row's maximum may pass the one that its weights
 // are relative to before they are scaled anew, in large blocks of rows: weights
-// stay below 2^8, and most steps need no pass over O (65.7 M vector
+// grow by 2^8 at most, and most steps need no pass over O (65.7 M vector
 // instructions, 57.4 with the slack, for 2047 tokens of 32 heads after 4000).  With
-// few rows maxima seldom grow, and without slack the largest weight is 1 and exact.
+// few rows maxima seldom grow, and there is no slack.
 constexpr float kSlack = 8.0f;
+
+// Weights are taken relative to a row's maximum plus this (in powers of two), so that the
+// sum of all of them stays at 1 at most: bf16's values reach 2^127.6, and a sum of them
+// that is divided at the end must not pass 32 bits' range before.  An addend of the
+// maximum, it costs nothing.  f16's values are far from there, and its weights
+// have no exponents to spare.
+template <typename T>
+__device__ __forceinline__ float headroom(int tokens, float slack) {
+    return __is_same(T, Bf16) ? (float)(32 - __builtin_clz((uint32_t)tokens | 1u)) + slack : 0.0f;
+}
 
 __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
 

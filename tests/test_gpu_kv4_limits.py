@@ -141,3 +141,32 @@ def test_attention_windows_that_hide_nothing(gpu, case, causal, window):
     cache, tables, lens_t, cu, q = scene
     got = _attend(scene, hk, max(qs), max_kv, causal, window)
     _check_attention(got, q, cache, tables, lens_t, cu, causal, 0, d ** -0.5)
+
+
+# ---- sums of large values ---------------------------------------------------------
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("ratio,n,max_kv", [(1, 1, 200), (4, 1, 600), (4, 1, 100000), (4, 5, 2_000_000), (8, 9, 2_000_000),
+                                            (32, 70, 2_000_000)])
+def test_attention_of_values_near_the_largest(gpu, d, ratio, n, max_kv):
+    """Values whose weighted sum is in range where the sum of their products with
+    weights that are not divided yet is not; and others that are all very small."""
+    lens, qs, ps = [700], [n], 16
+    cache, tables, lens_t, cu, q = _scene(torch.Generator().manual_seed(d), lens, qs, 2 * ratio, 2, d, ps, BF)
+    vs = plain.places(ps, d)[3]
+    for byte in (252, 45):
+        cache[:, :, vs] = byte
+        cache[:, :, vs[:, ::2]] = byte - 3
+        scene = cache, tables, lens_t, cu, q
+        got = _attend(scene, 2, n, max_kv)
+        assert torch.isfinite(got).all(), byte
+        _check_attention(got, q, cache, tables, lens_t, cu, True, 0, d ** -0.5)
+
+
+def test_attention_of_the_largest_value_everywhere(gpu):
+    lens, qs, ps, d = [3000, 20], [1, 1], 16, 128
+    cache, tables, lens_t, cu, q = _scene(torch.Generator().manual_seed(1), lens, qs, 8, 2, d, ps, BF, garbage=False)
+    cache[:, :, ps * d // 2:ps * d] = 0x77
+    cache[:, :, plain.places(ps, d)[3]] = 252
+    got = _attend((cache, tables, lens_t, cu, q), 2, 1, 3000).double()
+    most = 6 * 2.0 ** 125
+    assert ((got - most).abs() <= 2 * plain.half_step(BF) * most).all()
