@@ -855,6 +855,15 @@ bool large_blocks(int64_t blocks, int64_t seen, int D) {
     return blocks * seen >= (D == 64 ? 1500000 : D == 128 ? 550000 : 500000);
 }
 
+// A launch has less than 2^32 threads, 512 of a workgroup at most.
+constexpr int64_t kMaxGrid = 0x7fffff;
+
+// Whether blocks of 256 rows, the largest there are, are too many already: past this
+// the cut counts in 32 bits.
+bool past_a_launch(int num_seqs, int max_q, int ratio, int hk) {
+    return num_seqs && ((int64_t)max_q * ratio + 255) / 256 > kMaxGrid / ((int64_t)num_seqs * hk);
+}
+
 Cut cut_of(int num_seqs, int max_q, int64_t max_kv, int ratio, int hk, int D, int window) {
     Cut c{};
     const int64_t rows = (int64_t)max_q * ratio;
@@ -918,10 +927,10 @@ int32_t sizes_ok(int num_seqs, int total_q, int max_q, int64_t max_kv, int hq, i
     if (hq % hk) return kInvalid;
     if (!head_dim_ok(D) || !page_size_ok(ps) || element == kF32) return kUnsupported;
     if (num_pages > 0x7fffffff || max_kv > 0x7fffff00 || hq > 32768) return kUnsupported;
-    const Cut c = cut_of(num_seqs, max_q, max_kv, hq / hk, hk, D, window);
-    // a launch has less than 2^32 threads, 512 of a workgroup at most
-    if (c.grid > 0x7fffff) return kUnsupported;
-    return kOk;
+    // rows are counted in 32 bits, also those of a sequence that is longer than max_q
+    if ((int64_t)total_q * (hq / hk) > 0x7ffffc00) return kUnsupported;
+    if (past_a_launch(num_seqs, max_q, hq / hk, hk)) return kUnsupported;
+    return cut_of(num_seqs, max_q, max_kv, hq / hk, hk, D, window).grid > kMaxGrid ? kUnsupported : kOk;
 }
 
 }  // namespace
@@ -943,6 +952,7 @@ extern "C" size_t baracuda_kernels_kv4_attention_gfx950_workspace_size(int32_t n
                                                                        int32_t head_dim, int32_t window) {
     if (num_seqs < 1 || max_q < 1 || max_kv < 1 || num_kv_heads < 1 || num_heads < num_kv_heads || head_dim < 1 || window < 0)
         return 0;
+    if (past_a_launch(num_seqs, max_q, num_heads / num_kv_heads, num_kv_heads)) return 0;
     return cut_of(num_seqs, max_q, max_kv, num_heads / num_kv_heads, num_kv_heads, head_dim, window).bytes;
 }
 
