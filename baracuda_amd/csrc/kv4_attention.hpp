@@ -4,9 +4,10 @@
 //   o = softmax(scale q k^T + mask) v
 //
 // A sequence's new tokens are its last ones: token i of n stands at position
-// len - n + i.  A row (a token and a head) sees the positions up to its own
-// (all of the sequence without `causal`) and, with a window w, the last w of
-// those.  A row that sees nothing gives zeros.  Rows of one kv head are taken
+// len - n + i.  `causal` hides the positions after a row's own (a row is a token
+// and a head), a window w those that lie w or more before it, each by itself: a
+// row with both sees the last w positions up to its own, one with a window alone
+// those and all later ones.  A row that sees nothing gives zeros.  Rows of one kv head are taken
 // together: row r is token r / ratio and head r % ratio of the group.
 #pragma once
 

@@ -211,13 +211,15 @@ class Kv4AttentionDescriptor:
     max_pages: int                     # columns of the tables
     element: ElementKind = ElementKind.Bf16
     causal: bool = True
-    window: int = 0                    # 0: none
+    window: int = 0                    # positions that a row sees up to its own; 0: all
     scale: Optional[float] = None      # 1 / sqrt(head_dim)
 
 
 class Kv4AttentionPlan:
     """softmax(scale q K^T + mask) V over the pages of each sequence, whose new
-    tokens are its last ones.  A row that sees nothing gives zeros."""
+    tokens are its last ones.  `causal` hides what comes after a row's own
+    position, `window` what lies that far or further before it.  A row that sees
+    nothing gives zeros."""
 
     def __init__(self, desc: Kv4AttentionDescriptor):
         d = self.desc = desc

@@ -616,9 +616,10 @@ int32_t baracuda_kernels_kv4_read_gfx950_can_implement(
  * cache, a sequence's new ones being the last of them; tables int32 [num_seqs,
  * max_pages] (table_stride), a sequence's pages in order.  max_q and max_kv are
  * what the host knows of the lengths: rows past max_q of a sequence are not
- * computed, max_kv only decides how the work is cut.  With `causal` a row sees
- * the positions up to its own, with window > 0 the last `window` of those; a row
- * that sees nothing gives zeros.  An entry outside the cache stands for tokens
+ * computed, max_kv only decides how the work is cut.  `causal` hides the positions
+ * after a row's own, window > 0 those that lie `window` or more before it (each by
+ * itself: a window without `causal` leaves all later positions); a row that sees
+ * nothing gives zeros.  An entry outside the cache stands for tokens
  * that no row sees.  f16 and bf16; an f16 cache is one that f16 was appended to.
  * The workspace (16-byte aligned) is required where its size is not 0. */
 int32_t baracuda_kernels_kv4_attention_gfx950_run(

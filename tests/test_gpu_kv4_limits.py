@@ -5,7 +5,7 @@ import torch
 from baracuda_amd import kv4
 from tests import kv4_plain as plain
 from tests.gpu_util import sync
-from tests.test_gpu_kv4 import (BF, FL, KIND, _check_attention, _dev, _near, _on_gpu, _plain_rows, _rotation, _rows, _same,
+from tests.test_gpu_kv4 import (BF, FL, HF, KIND, _check_attention, _dev, _near, _on_gpu, _plain_rows, _rotation, _rows, _same,
                                 _scene)
 
 pytestmark = pytest.mark.gpu
@@ -141,6 +141,27 @@ def test_attention_windows_that_hide_nothing(gpu, case, causal, window):
     cache, tables, lens_t, cu, q = scene
     got = _attend(scene, hk, max(qs), max_kv, causal, window)
     _check_attention(got, q, cache, tables, lens_t, cu, causal, 0, d ** -0.5)
+
+
+@pytest.mark.parametrize("d,dt", [(64, HF), (128, BF), (256, BF)], ids=str)
+@pytest.mark.parametrize("seqs,max_q,max_kv", [(1, 1, 300), (1, 1, 100000), (2, 1, 600), (32, 20, 1100), (2, 64, 2_000_000)])
+def test_attention_window_without_causal(gpu, d, dt, seqs, max_q, max_kv):
+    """A window w hides what lies w or more positions before the row's own; the
+    positions after it are hidden by `causal` alone.  The same tokens are hidden here
+    by taking their pages out of the table, without a window."""
+    ps, hq, hk, n = 16, 8, 2, 3
+    lens, qs = [410] + [0] * (seqs - 1), [n] + [0] * (seqs - 1)
+    if max_q == 1:
+        n = qs[0] = 1
+    cache, tables, lens_t, cu, q = _scene(torch.Generator().manual_seed(d), lens, qs, hq, hk, d, ps, dt)
+    for i in range(n):           # row i stands at 410 - n + i: windows that begin with a page
+        first = 11 * ps
+        window = lens[0] - n + i - first + 1
+        got = _attend((cache, tables, lens_t, cu, q), hk, max_q, max_kv, causal=False, window=window)
+        cut = tables.clone()
+        cut[0, :11] = -1
+        one = torch.tensor([0, 1] + [1] * (seqs - 1), dtype=torch.int32)
+        _check_attention(got[i:i + 1], q[i:i + 1], cache, cut, lens_t, one, False, 0, d ** -0.5)
 
 
 # ---- sums of large values ---------------------------------------------------------
