@@ -24,7 +24,8 @@
  *     optional workspace (when given at least that size, 256- / 16-byte
  *     aligned; contents on entry do not matter) selects a faster path: the
  *     u8 pre-pass, the dense GEMV's split-K, the int8 tail round split along
- *X
+ *     K (two launches, bit-identical output).  Without it every entry point
+ *     but those two runs as-is.
  *
  * Each declaration cites the reference entry point it replaces
  * (paths relative to the baracuda repository root).
