@@ -173,8 +173,11 @@ __global__ __launch_bounds__(256) void fork_kernel(uint8_t *cache, int32_t *tabl
         const int64_t layer = rest / n;
         const int to = fresh[i];
         if (to < 0) continue;
-        const int p = parents[i];
-        const int from = tables[(int64_t)p * max_pages + lens[p] / ps];
+        // the parent's length is read again: should it be a child too, against what is
+        // asked of the caller, it may be another one by now, as long as the table
+        const int p = parents[i], last = lens[p] / ps;
+        if (last >= max_pages) continue;
+        const int from = tables[(int64_t)p * max_pages + last];
         if (from < 0 || from >= pages) continue;
         const int64_t at = part * span, bytes = page_bytes - at < span ? page_bytes - at : span;
         copy_span<V, false>(cache + (layer * pages + to) * page_bytes + at, cache + (layer * pages + from) * page_bytes + at, bytes);

@@ -191,3 +191,25 @@ def test_attention_of_the_largest_value_everywhere(gpu):
     got = _attend((cache, tables, lens_t, cu, q), 2, 1, 3000).double()
     most = 6 * 2.0 ** 125
     assert ((got - most).abs() <= 2 * plain.half_step(BF) * most).all()
+
+
+# ---- pages -------------------------------------------------------------------------
+@pytest.mark.parametrize("size", [32, 20000])
+def test_pages_fork_of_a_row_that_is_a_child_too(gpu, size):
+    """Which the caller must not ask for: what the two rows hold then is open, but nothing
+    past the tables is read and no page but the one handed out is written."""
+    g = torch.Generator().manual_seed(size)
+    cache = torch.randint(0, 256, (2, 9, size), generator=g, dtype=torch.uint8)
+    tables = torch.tensor([[0, 1], [-1, -1], [4, 5]], dtype=torch.int32)
+    lens, refs = torch.tensor([8, 0, 5], dtype=torch.int32), torch.tensor([1, 1, 0, 0, 1, 1, 0, 0, 0], dtype=torch.int32)
+    dev = [_dev(x) for x in (cache, tables, lens, refs)]
+    fresh = torch.empty(2, dtype=torch.int32, device=gpu)
+    # the last row is read by the first fork and becomes a full one by the second
+    kv4.KvPagesPlan.select(kv4.KvPagesDescriptor(2, 9, size, 4, 3, 2)).fork(
+        *dev, _dev(torch.tensor([2, 0], dtype=torch.int32)), _dev(torch.tensor([1, 2], dtype=torch.int32)), fresh)
+    sync()
+    assert fresh.tolist() == [2, -1]
+    got = dev[0].cpu()
+    rest = [p for p in range(9) if p != 2]
+    _same(got[:, rest], cache[:, rest], "pages")
+    assert int(dev[1].min()) >= -1 and int(dev[1].max()) < 9 and dev[1][0].tolist() == [0, 1] and int(dev[3].min()) >= 0
