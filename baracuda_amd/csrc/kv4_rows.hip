@@ -13,19 +13,20 @@
 // A lane holds eight values, a head D / 8 lanes.  A token's cosines and sines
 // come through LDS once, and a wave has up to six rounds of heads of one token, all
 // loaded before the first is used.  Bound by HBM, with the vector unit close behind:
-// 6145 tokens of 40 heads of 128, three position axes, 129 MB in 33.5 us (3.9 TB/s;
-// a large copy 4.8), 21 us of them vector instructions' issue.  What it took: heads
+// 6145 tokens of 40 heads of 128, three position axes, 129 MB in 36 us (3.5 TB/s;
+// a large copy 4.8), 22 us of them vector instructions' issue.  What it took: heads
 // of all kinds in one wave and the table read by every lane 132 us; the table
 // through LDS, three rounds a wave 53; rounds of one kind, norm's and rotation's
-// factors multiplied once 36; six rounds 33.5 (twelve 33.8).  8191 tokens of 16 + 4
-// heads of 256 into the cache: 156 MB in 46 us.
+// factors multiplied once 36; six rounds 33.5 (twelve 33.8); a look at whether 32
+// bits held what came out, 1.9 more.  8191 tokens of 16 + 4 heads of 256 into the cache:
+// 157 MB in 47 us, of which a wave waits 60%: its workgroup loads two tokens, meets a
+// barrier, stores and ends.
 //
-// Q, and K without a cache, are computed in 32 bits and rounded once (heads that
-// leave their range, in 64).  K that
-// is quantized is computed in 64 bits: it is rounded to the element's type
-// first and then to 4 bits, and a value next to a border between two codes has
-// to fall on the side of the exact one, or equal prefixes would give unequal
-// pages.
+// Q, and K without a cache, are computed in 32 bits and rounded once; heads that
+// leave their range, in 64.  K that is quantized is computed in 64 bits: it is
+// rounded to the element's type first and then to 4 bits, and a value next to a
+// border between two codes has to fall on the side of the exact one, or equal
+// prefixes would give unequal pages.
 #include "kv4.hpp"
 
 namespace bk {
@@ -337,8 +338,9 @@ __global__ __launch_bounds__(64 * kWaves) void rows_kernel(const RowArgs a, int 
 }
 
 // A lane reads eight values of K or V of one token; slots out of range read as
-// zeros.  A workgroup has `several` tokens, or part of one.  Bound by the writes:
-// 8191 tokens of 2 heads of 256, 21 MB in 7.3 us.
+// zeros.  A workgroup has `several` tokens, or part of one.  Bound by its chain of loads,
+// slot, then code and scale, before the one store of a lane: 8191 tokens of 2 heads of
+// 256, 21 MB in 7.2 us (2.9 TB/s), half of a wave's time waited.
 template <typename T>
 __global__ __launch_bounds__(256) void read_kernel(const uint8_t *__restrict__ cache, const int64_t *__restrict__ slots,
                                                    int64_t tokens, int64_t num_slots, void *k_out, int64_t k_token,

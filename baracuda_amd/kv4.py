@@ -89,8 +89,8 @@ class QkNormRopeDescriptor:
 
 class QkNormRopePlan:
     """q_out, k_out = rotate(x * w / sqrt(mean(x^2) + eps)) of each head, in one
-    pass.  Statistics and products are held in 32 bits and rounded once; the
-    outputs may be the inputs."""
+    pass.  Statistics and products are held in 32 bits (in 64 for heads that leave
+    their range) and rounded once; the outputs may be the inputs."""
 
     def __init__(self, desc: QkNormRopeDescriptor):
         d = self.desc = desc
