@@ -23,10 +23,9 @@ LIB = PKG / "libbaracuda_kernels.so"
 # Measurement kernels of bench.py (not product), built beside the library.
 PROBES = PKG / "probes"
 PROBE_LIB = PKG / "libbaracuda_probes.so"
-# The plans' calls of the 4-bit cache's entry points, a Python module over torch's
-# headers (host code), beside the library that it calls.
-BINDING_SRC = CSRC / "kv4_binding.cpp"
-BINDING = PKG / "_kv4.so"
+# The calls of the plans of ``kv4`` and ``w4``, Python modules over torch's headers
+# (host code), beside the library that they call: csrc/<name>_binding.cpp, _<name>.so.
+BINDINGS = {CSRC / "kv4_binding.cpp": PKG / "_kv4.so", CSRC / "w4_binding.cpp": PKG / "_w4.so"}
 # Digest of the sources and flags the library was built from, written beside it.
 STAMP = PKG / "libbaracuda_kernels.so.srchash"
 
@@ -71,7 +70,7 @@ def source_digest() -> str:
 
 def is_stale() -> bool:
     """True when the library is missing or was built from other sources."""
-    if not LIB.exists() or not BINDING.exists() or not STAMP.exists() or (any(PROBES.glob("*.hip")) and not PROBE_LIB.exists()):
+    if not LIB.exists() or not all(b.exists() for b in BINDINGS.values()) or not STAMP.exists() or (any(PROBES.glob("*.hip")) and not PROBE_LIB.exists()):
         return True
     return STAMP.read_text().strip() != source_digest()
 
@@ -97,33 +96,33 @@ def _build_probes() -> None:
     os.replace(tmp, PROBE_LIB)
 
 
-def _compile_binding() -> Path:
+def _compile_binding(src: Path) -> Path:
     import sysconfig
 
     import torch
     from torch.utils.cpp_extension import include_paths
 
-    obj = BUILD / "kv4_binding.o"
+    obj = BUILD / (src.stem + ".o")
     dirs = [*include_paths(), sysconfig.get_paths()["include"], str(ROOT / "include")]
     cmd = [CXX, "-O2", "-std=c++17", "-fPIC", "-fvisibility=hidden",
            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", *(f"-I{d}" for d in dirs),
-           "-c", str(BINDING_SRC), "-o", str(obj)]
+           "-c", str(src), "-o", str(obj)]
     res = subprocess.run(cmd, capture_output=True, text=True)
     if res.returncode != 0:
-        raise RuntimeError(f"{CXX} failed for {BINDING_SRC.name}:\n{res.stderr}")
+        raise RuntimeError(f"{CXX} failed for {src.name}:\n{res.stderr}")
     return obj
 
 
-def _link_binding(obj: Path) -> None:
+def _link_binding(obj: Path, binding: Path) -> None:
     import torch
 
-    tmp = BINDING.with_suffix(".so.tmp")
+    tmp = binding.with_suffix(".so.tmp")
     cmd = [CXX, "-shared", str(obj), f"-L{PKG}", "-l:libbaracuda_kernels.so", "-Wl,-rpath,$ORIGIN",
            f"-L{Path(torch.__file__).parent / 'lib'}", "-ltorch_python", "-ltorch_cpu", "-lc10", "-o", str(tmp)]
     res = subprocess.run(cmd, capture_output=True, text=True)
     if res.returncode != 0:
-        raise RuntimeError(f"link failed for {BINDING.name}:\n{res.stderr}")
-    os.replace(tmp, BINDING)
+        raise RuntimeError(f"link failed for {binding.name}:\n{res.stderr}")
+    os.replace(tmp, binding)
 
 
 def build(verbose: bool = False) -> Path:
@@ -132,7 +131,7 @@ def build(verbose: bool = False) -> Path:
     digest = source_digest()
     sources = sorted(CSRC.glob("*.hip"))
     with cf.ThreadPoolExecutor(max_workers=min(8, len(sources))) as ex:
-        binding = ex.submit(_compile_binding)
+        bindings = {ex.submit(_compile_binding, src): out for src, out in BINDINGS.items()}
         objs = list(ex.map(_compile, sources))
     tmp = LIB.with_suffix(".so.tmp")
     cmd = [HIPCC, f"--offload-arch={ARCH}", "-shared", "-fPIC", *map(str, objs), "-o", str(tmp)]
@@ -140,7 +139,8 @@ def build(verbose: bool = False) -> Path:
     if res.returncode != 0:
         raise RuntimeError(f"link failed:\n{res.stderr}")
     os.replace(tmp, LIB)
-    _link_binding(binding.result())
+    for obj, out in bindings.items():
+        _link_binding(obj.result(), out)
     _build_probes()
     STAMP.write_text(digest + "\n")
     if verbose:

@@ -1,30 +1,9 @@
 // kv4_binding.cpp -- the plans' calls of the 4-bit cache's entry points.
-//
-// A step of a decoding loop runs kernels of a few microseconds, so what is done
-// for each call before the launch counts as much as they do: the checks of ten
-// operands and a call of thirty arguments take 10 to 20 us in Python and 1 us
-// here.  Every function takes a plan's sizes (packed 8-byte values), the stream
-// (None: torch's current one) and the operands, checks the operands against the
-// sizes, raises InvalidProblem as the other plans do, and returns the status of
-// the one C entry point that it calls.
-#include <torch/csrc/autograd/python_variable.h>
-
-#include <cstdint>
-#include <cstring>
-
-#include "baracuda_kernels.h"
+#include "binding.hpp"
 
 namespace {
 
-PyObject *g_invalid = nullptr;      // plans.InvalidProblem
-PyObject *g_raw_stream = nullptr;   // device index -> the current stream's handle
-
-struct Raised {};
-
-[[noreturn]] void refuse(const char *what, const char *why) {
-    PyErr_Format(g_invalid, "%s %s", what, why);
-    throw Raised{};
-}
+using namespace binding;
 
 // The sizes that every plan packs, in this order; what a plan has no use for is 0.
 struct Sizes {
@@ -35,29 +14,9 @@ struct Sizes {
     int64_t layers, page_bytes, rows;
 };
 
-class Call {
+class Call : public Operands<Sizes> {
 public:
-    Call(PyObject *const *args, Py_ssize_t n, Py_ssize_t want) : args_(args + 2), stream_(args[1]) {
-        if (n != want + 2 || !PyBytes_Check(args[0]) || PyBytes_GET_SIZE(args[0]) != (Py_ssize_t)sizeof(Sizes)) {
-            PyErr_SetString(PyExc_TypeError, "a plan's sizes, a stream and its operands");
-            throw Raised{};
-        }
-        std::memcpy(&s, PyBytes_AS_STRING(args[0]), sizeof(Sizes));
-        dtype = s.element == 0 ? at::kFloat : s.element == 1 ? at::kHalf : at::kBFloat16;
-    }
-
-    bool given(int i) const { return args_[i] != Py_None; }
-
-    const at::Tensor &tensor(int i, const char *what) {
-        PyObject *o = args_[i];
-        if (o == Py_None) refuse(what, "is required");
-        if (!THPVariable_Check(o)) refuse(what, "must be a tensor");
-        const at::Tensor &t = THPVariable_Unpack(o);
-        if (!t.is_cuda()) host_ = true;
-        else if (device_ < 0) device_ = t.get_device();
-        else if (device_ != t.get_device()) refuse(what, "must be on the GPU of the other operands");
-        return t;
-    }
+    using Operands::Operands;
 
     struct Rows {
         void *p = nullptr;
@@ -80,32 +39,12 @@ public:
         return Rows{t.data_ptr(), t0, t1};
     }
 
-    // A dense tensor of one dimension or two (columns < 0: one).
-    template <typename P>
-    P *dense(int i, const char *what, at::ScalarType type, int64_t n, int64_t columns = -1) {
-        const at::Tensor &t = tensor(i, what);
-        const bool shape = columns < 0 ? t.dim() == 1 && t.size(0) == n : t.dim() == 2 && t.size(0) == n && t.size(1) == columns;
-        if (!shape) refuse(what, "does not have the descriptor's sizes");
-        if (t.scalar_type() != type) refuse(what, "is of another type");
-        if (!t.is_contiguous()) refuse(what, "must be contiguous");
-        return (P *)t.data_ptr();
-    }
-
     void *cache(int i, int64_t a, int64_t b, int64_t c, bool any_byte) {
         const at::Tensor &t = tensor(i, "cache");
         if (t.dim() != 3 || t.size(0) != a || t.size(1) != b || t.size(2) != c)
             refuse("cache", "does not have the descriptor's sizes");
         if (any_byte ? t.element_size() != 1 : t.scalar_type() != at::kByte) refuse("cache", "must be bytes");
         if (!t.is_contiguous()) refuse("cache", "must be contiguous");
-        return t.data_ptr();
-    }
-
-    void *workspace(int i, size_t &bytes) {
-        bytes = 0;
-        if (!given(i)) return nullptr;
-        const at::Tensor &t = tensor(i, "workspace");
-        if (!t.is_contiguous()) refuse("workspace", "must be contiguous");
-        bytes = t.nbytes();
         return t.data_ptr();
     }
 
@@ -143,57 +82,11 @@ public:
         else if (given(i + 5)) refuse("pair_axis:", "one axis takes none");
         return r;
     }
-
-    // After all operands: they are on a GPU, and this is its stream.
-    void *stream() {
-        if (host_ || device_ < 0) refuse("operand tensors", "must be on the GPU");
-        PyObject *v = nullptr;
-        if (stream_ == Py_None) {
-            PyObject *index = PyLong_FromLong(device_);
-            v = index ? PyObject_CallFunctionObjArgs(g_raw_stream, index, nullptr) : nullptr;
-            Py_XDECREF(index);
-        } else if (PyLong_Check(stream_)) {
-            Py_INCREF(stream_);
-            v = stream_;
-        } else {
-            v = PyObject_GetAttrString(stream_, "cuda_stream");
-        }
-        if (!v) throw Raised{};
-        void *h = PyLong_AsVoidPtr(v);
-        Py_DECREF(v);
-        if (!h && PyErr_Occurred()) throw Raised{};
-        return h;
-    }
-
-    Sizes s;
-    at::ScalarType dtype;
-
-private:
-    PyObject *const *args_;
-    PyObject *stream_;
-    int device_ = -1;
-    bool host_ = false;
 };
-
-template <int N, typename F>
-PyObject *guarded(PyObject *const *args, Py_ssize_t n, F f) {
-    try {
-        Call c(args, n, N);
-        return PyLong_FromLong(f(c));
-    } catch (const Raised &) {
-        return nullptr;
-    } catch (const std::exception &e) {
-        PyErr_SetString(PyExc_RuntimeError, e.what());
-        return nullptr;
-    } catch (...) {
-        PyErr_SetString(PyExc_RuntimeError, "unknown exception");
-        return nullptr;
-    }
-}
 
 // q, k, q_out, k_out, q_weight, k_weight, positions, cos, sin, pair_axis
 PyObject *qk_norm_rope(PyObject *, PyObject *const *args, Py_ssize_t n) {
-    return guarded<10>(args, n, [](Call &c) {
+    return guarded<Call, 10>(args, n, [](Call &c) {
         const Sizes &s = c.s;
         const auto q = c.rows(0, "q", s.tokens, s.hq, false), k = c.rows(1, "k", s.tokens, s.hk, false);
         const auto qo = c.rows(2, "q_out", s.tokens, s.hq, true), ko = c.rows(3, "k_out", s.tokens, s.hk, true);
@@ -210,7 +103,7 @@ int64_t head_bytes(const Sizes &s) { return s.ps * (s.D + s.D / 16); }
 
 // k, v, cache, slots, q, q_out, q_weight, k_weight, positions, cos, sin, pair_axis
 PyObject *append(PyObject *, PyObject *const *args, Py_ssize_t n) {
-    return guarded<12>(args, n, [](Call &c) {
+    return guarded<Call, 12>(args, n, [](Call &c) {
         const Sizes &s = c.s;
         const auto k = c.rows(0, "k", s.tokens, s.hk, false), v = c.rows(1, "v", s.tokens, s.hk, false);
         void *cache = c.cache(2, s.pages, s.hk, head_bytes(s), false);
@@ -229,7 +122,7 @@ PyObject *append(PyObject *, PyObject *const *args, Py_ssize_t n) {
 
 // cache, slots, k_out, v_out
 PyObject *read(PyObject *, PyObject *const *args, Py_ssize_t n) {
-    return guarded<4>(args, n, [](Call &c) {
+    return guarded<Call, 4>(args, n, [](Call &c) {
         const Sizes &s = c.s;
         void *cache = c.cache(0, s.pages, s.hk, head_bytes(s), false);
         const int64_t *slots = c.dense<int64_t>(1, "slots", at::kLong, s.tokens);
@@ -242,7 +135,7 @@ PyObject *read(PyObject *, PyObject *const *args, Py_ssize_t n) {
 
 // q, cache, tables, kv_lens, out, cu_q, workspace
 PyObject *attention(PyObject *, PyObject *const *args, Py_ssize_t n) {
-    return guarded<7>(args, n, [](Call &c) {
+    return guarded<Call, 7>(args, n, [](Call &c) {
         const Sizes &s = c.s;
         const auto q = c.rows(0, "q", s.tokens, s.hq, false);
         void *cache = c.cache(1, s.pages, s.hk, head_bytes(s), false);
@@ -267,7 +160,7 @@ PyObject *attention(PyObject *, PyObject *const *args, Py_ssize_t n) {
 
 // cache, src, dst
 PyObject *pages_copy(PyObject *, PyObject *const *args, Py_ssize_t n) {
-    return guarded<3>(args, n, [](Call &c) {
+    return guarded<Call, 3>(args, n, [](Call &c) {
         const Sizes &s = c.s;
         void *cache = c.cache(0, s.layers, s.pages, s.page_bytes, true);
         const at::Tensor &t = c.tensor(1, "src");
@@ -280,7 +173,7 @@ PyObject *pages_copy(PyObject *, PyObject *const *args, Py_ssize_t n) {
 
 // cache, tables, lens, refs, parents, children, fresh
 PyObject *pages_fork(PyObject *, PyObject *const *args, Py_ssize_t n) {
-    return guarded<7>(args, n, [](Call &c) {
+    return guarded<Call, 7>(args, n, [](Call &c) {
         const Sizes &s = c.s;
         void *cache = c.cache(0, s.layers, s.pages, s.page_bytes, true);
         int32_t *tables = c.dense<int32_t>(1, "tables", at::kInt, s.rows, s.max_pages);
@@ -299,7 +192,7 @@ PyObject *pages_fork(PyObject *, PyObject *const *args, Py_ssize_t n) {
 
 // tables, lens, refs, rows
 PyObject *pages_release(PyObject *, PyObject *const *args, Py_ssize_t n) {
-    return guarded<4>(args, n, [](Call &c) {
+    return guarded<Call, 4>(args, n, [](Call &c) {
         const Sizes &s = c.s;
         int32_t *tables = c.dense<int32_t>(0, "tables", at::kInt, s.rows, s.max_pages);
         int32_t *lens = c.dense<int32_t>(1, "lens", at::kInt, s.rows), *refs = c.dense<int32_t>(2, "refs", at::kInt, s.pages);
@@ -315,7 +208,7 @@ PyObject *pages_release(PyObject *, PyObject *const *args, Py_ssize_t n) {
 
 // cache, tables, refs, tables_out, refs_out, remap, live, workspace
 PyObject *pages_compact(PyObject *, PyObject *const *args, Py_ssize_t n) {
-    return guarded<8>(args, n, [](Call &c) {
+    return guarded<Call, 8>(args, n, [](Call &c) {
         const Sizes &s = c.s;
         void *cache = c.cache(0, s.layers, s.pages, s.page_bytes, true);
         const int32_t *tables = c.dense<int32_t>(1, "tables", at::kInt, s.rows, s.max_pages);
@@ -332,26 +225,10 @@ PyObject *pages_compact(PyObject *, PyObject *const *args, Py_ssize_t n) {
     });
 }
 
-// The exception that refusals raise, and torch's lookup of the current stream.
-PyObject *connect(PyObject *, PyObject *const *args, Py_ssize_t n) {
-    if (n != 2) {
-        PyErr_SetString(PyExc_TypeError, "connect(exception, raw_stream)");
-        return nullptr;
-    }
-    Py_INCREF(args[0]);
-    Py_INCREF(args[1]);
-    Py_XDECREF(g_invalid);
-    Py_XDECREF(g_raw_stream);
-    g_invalid = args[0], g_raw_stream = args[1];
-    Py_RETURN_NONE;
-}
-
-#define BK_METHOD(NAME) {#NAME, (PyCFunction)(void (*)(void))NAME, METH_FASTCALL, nullptr}
 PyMethodDef kMethods[] = {BK_METHOD(connect),       BK_METHOD(qk_norm_rope), BK_METHOD(append),
                           BK_METHOD(read),          BK_METHOD(attention),    BK_METHOD(pages_copy),
                           BK_METHOD(pages_fork),    BK_METHOD(pages_release), BK_METHOD(pages_compact),
                           {nullptr, nullptr, 0, nullptr}};
-#undef BK_METHOD
 
 PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "_kv4", nullptr, -1, kMethods, nullptr, nullptr, nullptr, nullptr};
 

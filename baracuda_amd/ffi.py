@@ -157,6 +157,19 @@ _sig("baracuda_kernels_kv_pages_compact_gfx950_run", i32, *_KV_PAGES, vp, vp, vp
 _sig("baracuda_kernels_kv_pages_gfx950_workspace_size", sz, *_KV_PAGES)
 _sig("baracuda_kernels_kv_pages_gfx950_can_implement", i32, *_KV_PAGES)
 
+_sig("baracuda_kernels_w4_packed_bytes_gfx950", sz, i32, i32)
+_sig("baracuda_kernels_w4_quantize_gfx950_run", i32, i32, i32, i32, i32, vp, i64, i64, vp, vp)
+_sig("baracuda_kernels_w4_pack_gfx950_run", i32, i32, i32, i32, vp, vp, vp, vp)
+_sig("baracuda_kernels_w4_read_gfx950_run", i32, i32, i32, i32, i32, vp, vp, i64, i64, vp)
+_sig("baracuda_kernels_w4_weights_gfx950_can_implement", i32, i32, i32, i32, i32)
+_W4 = (i32, i32, i32, i32, i32)               # m, n, k, element, gated
+_sig("baracuda_kernels_w4_linear_gfx950_run", i32, *_W4, vp, i64, vp, vp, vp, i64, vp, sz, vp)
+_sig("baracuda_kernels_w4_linear_gfx950_can_implement", i32, *_W4)
+_sig("baracuda_kernels_w4_linear_gfx950_workspace_size", sz, *_W4)
+_sig("baracuda_kernels_moe_w4_grouped_gfx950_run", i32, i32, i32, *_W4, *(vp,) * 10, sz, vp)
+_sig("baracuda_kernels_moe_w4_grouped_gfx950_can_implement", i32, i32, i32, *_W4)
+_sig("baracuda_kernels_moe_w4_grouped_gfx950_workspace_size", sz, i32, i32, *_W4)
+
 SYMBOLS = tuple(_SIGS)
 
 _lib = None

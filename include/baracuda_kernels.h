@@ -674,6 +674,69 @@ size_t baracuda_kernels_kv_pages_gfx950_workspace_size(int32_t layers, int64_t n
 int32_t baracuda_kernels_kv_pages_gfx950_can_implement(int32_t layers, int64_t num_pages, int64_t page_bytes,
                                                        int32_t page_size, int32_t rows, int32_t max_pages);
 
+/* ======================= products with 4-bit weights =====================
+ * No counterpart in the reference: linear products whose weights are 4-bit codes
+ * under group scales, for one token, a few or a prompt, the same by expert, and
+ * what makes and reads such weights.  `element`: 0 f32, 1 f16, 2 bf16.
+ *
+ * A weight is code * 2^(byte - 127): a code is sign, two exponent bits, one mantissa
+ * bit (0, 0.5, 1, 1.5, 2, 3, 4, 6); 32 consecutive weights of a row share a byte,
+ * and byte 255 marks a group that held an infinity or a NaN and reads as NaN.  K is
+ * a multiple of 32.  A packed matrix [N, K] is w4_packed_bytes(N, K) bytes, 16-byte
+ * aligned:
+ *   codes   [ceil(N / 32)][tiles][64][16]           tiles = 2 ceil(K / 128)
+ *   scales  [ceil(N / 32)][ceil(K / 256)][64][4]
+ * Lane l of tile t holds row 32 b + l % 32, values 64 t + 32 (l / 32) .. + 31, two
+ * codes a byte, the lower index in the lower four bits; byte j of a lane's scales is
+ * that of tile 4 s + j.  Rows past N and values past K are zeros.  Several matrices
+ * lie one after the other. */
+size_t baracuda_kernels_w4_packed_bytes_gfx950(int32_t n, int32_t k);
+
+/* Weights [matrices, N, K] (strides in elements, K dense) to packed ones: the scale
+ * is the smallest power of two under which no magnitude of the group reaches 7 (of
+ * 2^-125 to 2^125; f16: up to 2^13, so that every weight is an f16), codes are the
+ * nearest, ties to the even code. */
+int32_t baracuda_kernels_w4_quantize_gfx950_run(int32_t matrices, int32_t n, int32_t k, int32_t element, const void *weights,
+                                                int64_t matrix_stride, int64_t row_stride, void *packed, void *stream);
+/* codes uint8 [matrices, N, K / 2] and scales uint8 [matrices, N, K / 32], as a
+ * checkpoint holds them, to packed weights. */
+int32_t baracuda_kernels_w4_pack_gfx950_run(int32_t matrices, int32_t n, int32_t k, const void *codes, const void *scales,
+                                            void *packed, void *stream);
+/* The values of packed weights, rounded to the element. */
+int32_t baracuda_kernels_w4_read_gfx950_run(int32_t matrices, int32_t n, int32_t k, int32_t element, const void *packed,
+                                            void *weights, int64_t matrix_stride, int64_t row_stride, void *stream);
+int32_t baracuda_kernels_w4_weights_gfx950_can_implement(int32_t matrices, int32_t n, int32_t k, int32_t element);
+
+/* y[m, n] = sum_k x[m, k] w[n, k] + bias[n] (f32 [N], may be NULL); out = y, or, gated
+ * != 0, silu(y[m, n]) * y[m, n + N / 2] for n < N / 2 (N a multiple of 64).  x, out
+ * f16 or bf16; sums, bias and gate in 32 bits, rounded once.  Weights enter as
+ * elements: exactly in bf16 for scales of 2^-125 to 2^125, in f16 for scales of 2^-23
+ * to 2^13, beyond that rounded to the element.  x is 16-byte aligned, ldx a multiple
+ * of 8. */
+int32_t baracuda_kernels_w4_linear_gfx950_run(int32_t m, int32_t n, int32_t k, int32_t element, int32_t gated, const void *x,
+                                              int64_t ldx, const void *packed, const float *bias, void *out, int64_t ldo,
+                                              void *workspace, size_t workspace_bytes, void *stream);
+int32_t baracuda_kernels_w4_linear_gfx950_can_implement(int32_t m, int32_t n, int32_t k, int32_t element, int32_t gated);
+size_t baracuda_kernels_w4_linear_gfx950_workspace_size(int32_t m, int32_t n, int32_t k, int32_t element, int32_t gated);
+
+/* The same by expert, for size_m token-expert pairs: position p holds pair id =
+ * sorted_token_ids[p] of expert expert_ids[p], positions in ascending order of the
+ * experts.  Input row id / topk (id when topk_weights != NULL), output row id:
+ * out[id] = end(x[row] W_e^T + bias[e]) [* topk_weights[id]], rounded once.  x has
+ * ceil(size_m / topk) rows (size_m when topk_weights != NULL), packed [E] matrices,
+ * bias f32 [E, N] or NULL.  expert_counts [E] and expert_offsets [E + 1] are filled by
+ * the call.  Positions whose expert is num_experts or more, all of them last, and ids
+ * outside the pairs are left out: nothing is written for them. */
+int32_t baracuda_kernels_moe_w4_grouped_gfx950_run(
+    int32_t num_experts, int32_t topk, int32_t size_m, int32_t n, int32_t k, int32_t element, int32_t gated, const void *x,
+    const void *packed, const int32_t *sorted_token_ids, const int32_t *expert_ids, const float *topk_weights,
+    const float *bias, void *out, int32_t *expert_counts, int32_t *expert_offsets, void *workspace, size_t workspace_bytes,
+    void *stream);
+int32_t baracuda_kernels_moe_w4_grouped_gfx950_can_implement(int32_t num_experts, int32_t topk, int32_t size_m, int32_t n,
+                                                             int32_t k, int32_t element, int32_t gated);
+size_t baracuda_kernels_moe_w4_grouped_gfx950_workspace_size(int32_t num_experts, int32_t topk, int32_t size_m, int32_t n,
+                                                             int32_t k, int32_t element, int32_t gated);
+
 #ifdef __cplusplus
 }
 #endif
