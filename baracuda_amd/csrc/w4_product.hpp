@@ -3,6 +3,7 @@
 #pragma once
 
 #include "w4.hpp"
+#include "w4_rules.hpp"
 
 namespace bk {
 namespace w4 {
@@ -16,9 +17,10 @@ struct ProductArgs {
     int64_t matrix;              // bytes of a packed matrix
     int M, N, K, tiles, words;
     // by expert: position p of the pairs sorted by expert has pair order[p]
-    const int32_t *order, *offsets;
+    const int32_t *order, *offsets, *expert_ids;     // offsets null: few pairs, from the ids
+    int32_t *counts_out, *offsets_out;
     const float *topk_weights;   // [size_m] by pair, or null
-    int E, size_m, in_div;       // input row of a pair: pair / in_div
+    int E, size_m, in_div;       // size_m: pairs, or M; input row of a pair: pair / in_div
 };
 
 // Rows of one workgroup: its rows of the list (a matrix's own rows, or positions
@@ -58,6 +60,84 @@ __device__ __forceinline__ bool expert_rows(const ProductArgs &a, int slot, Rows
     return false;
 }
 
+// Tiles of TB rows in all, as every lane's value.
+template <int TB>
+__device__ __forceinline__ int expert_tiles(const ProductArgs &a) {
+    const int lane = threadIdx.x & 63;
+    int n = 0;
+    for (int x = lane; x < a.E; x += 64) {
+        const int o0 = min(max(a.offsets[x], 0), a.size_m);
+        n += (max(min(a.offsets[x + 1], a.size_m) - o0, 0) + TB - 1) / TB;
+    }
+#pragma unroll
+    for (int off = 1; off < 64; off <<= 1) n += __shfl_xor(n, off, 64);
+    return __builtin_amdgcn_readfirstlane(n);
+}
+
+// The same for at most kFewPairs pairs from the ids themselves, which
+// saves the launch in front that counts them.
+constexpr int kFewPairs = 256;
+template <int TB>
+__device__ __forceinline__ bool expert_rows_few(const ProductArgs &a, int slot, Rows &r) {
+    constexpr int CHUNKS = kFewPairs / 64;
+    const int lane = threadIdx.x & 63;
+    int id[CHUNKS];
+    uint64_t head[CHUNKS];                 // positions whose expert is not the one before
+#pragma unroll
+    for (int i = 0; i < CHUNKS; ++i) id[i] = 64 * i + lane < a.size_m ? a.expert_ids[64 * i + lane] : -1;
+#pragma unroll
+    for (int i = 0; i < CHUNKS; ++i) {
+        const int before = i ? __builtin_amdgcn_readlane(id[i ? i - 1 : 0], 63) : -2, up = __shfl_up(id[i], 1, 64);
+        head[i] = __ballot(id[i] != (lane ? up : before));
+    }
+    int from = 0;                          // where the run that reaches into this chunk began
+#pragma unroll
+    for (int i = 0; i < CHUNKS; ++i) {
+        const uint64_t upto = head[i] & (~0ull >> (63 - lane));
+        const int began = upto ? 64 * i + 63 - __clzll((long long)upto) : from;
+        const uint64_t starts = __ballot((unsigned)id[i] < (unsigned)a.E && (64 * i + lane - began) % TB == 0);
+        const int n = __popcll(starts);
+        if (slot < n) {
+            const bool me = (starts >> lane & 1) && __popcll(starts & ((1ull << lane) - 1)) == slot;
+            const int l = __builtin_amdgcn_readfirstlane(__ffsll((unsigned long long)__ballot(me)) - 1);
+            r.e = __builtin_amdgcn_readlane(id[i], l);
+            r.first = 64 * i + l;
+            const uint64_t later = l < 63 ? head[i] >> (l + 1) : 0, next = i + 1 < CHUNKS ? head[i + 1 < CHUNKS ? i + 1 : 0] : 1;
+            // a run of more than TB goes on in another tile, so what lies in the next chunk is enough
+            const int run = later ? __ffsll((unsigned long long)later) : 64 - l + (next ? __ffsll((unsigned long long)next) - 1 : 64);
+            r.rows = min(min(TB, run), a.size_m - r.first);
+            return true;
+        }
+        slot -= n;
+        if (head[i]) from = 64 * i + 63 - __clzll((long long)head[i]);
+    }
+    return false;
+}
+
+// expert_counts and expert_offsets of few pairs, by one whole workgroup, through
+// kFewPairs words of LDS.
+__device__ __forceinline__ void count_experts(const ProductArgs &a, uint32_t *ids) {
+    __syncthreads();
+    for (int i = threadIdx.x; i < a.size_m; i += blockDim.x) ids[i] = (uint32_t)a.expert_ids[i];
+    __syncthreads();
+    const auto before = [&](uint32_t e) {      // positions of experts below e
+        int lo = 0, n = a.size_m;
+        while (n > 0) {
+            const int half = n / 2;
+            const bool below = ids[lo + half] < e;
+            lo = below ? lo + half + 1 : lo;
+            n = below ? n - half - 1 : half;
+        }
+        return lo;
+    };
+    for (int e = threadIdx.x; e < a.E; e += blockDim.x) {
+        const int first = before(e), last = before(e + 1);
+        a.counts_out[e] = last - first;
+        a.offsets_out[e] = first;
+        if (e == a.E - 1) a.offsets_out[a.E] = last;
+    }
+}
+
 // Input and output row of row r of a workgroup's; negative where there is none.
 template <bool MOE>
 __device__ __forceinline__ void row_of(const ProductArgs &a, const Rows &w, int r, int &in, int &out) {
@@ -75,6 +155,10 @@ __device__ __forceinline__ void row_of(const ProductArgs &a, const Rows &w, int 
 // below -88, and the quotient is then -0, as it should be.
 __device__ __forceinline__ float gated(float gate, float up) { return gate / (1.0f + __expf(-gate)) * up; }
 
+struct __attribute__((packed, aligned(2))) Unaligned8 {
+    v2i v;
+};
+
 // The end of a product: four consecutive columns from n of an output row, bias and
 // gate added in 32 bits and rounded once.  ncols: columns of the output.
 template <bool BF16>
@@ -83,8 +167,8 @@ __device__ __forceinline__ void store4(const ProductArgs &a, int row, int n, int
     uint32_t lo, hi;
     if constexpr (BF16) lo = f32x2_to_bf16x2(y[0], y[1]), hi = f32x2_to_bf16x2(y[2], y[3]);
     else lo = kv4::f32x2_to_f16x2(y[0], y[1]), hi = kv4::f32x2_to_f16x2(y[2], y[3]);
-    if (n + 4 <= ncols && ((uintptr_t)p & 7) == 0) {
-        *(v2i *)p = v2i{(int)lo, (int)hi};
+    if (n + 4 <= ncols) {
+        ((Unaligned8 *)p)->v = v2i{(int)lo, (int)hi};
         return;
     }
     const uint16_t h[4] = {(uint16_t)lo, (uint16_t)(lo >> 16), (uint16_t)hi, (uint16_t)(hi >> 16)};
@@ -103,6 +187,9 @@ __device__ __forceinline__ v4f bias4(const ProductArgs &a, int e, int n) {
     }
     return b;
 }
+
+int32_t launch_rows(const ProductArgs &a, bool bf16, bool moe, bool gated, hipStream_t stream);
+int32_t launch_tiles(const ProductArgs &a, bool bf16, bool moe, bool gated, hipStream_t stream);
 
 }  // namespace w4
 }  // namespace bk
