@@ -87,8 +87,14 @@ int32_t baracuda_kernels_moe_w4_grouped_gfx950_run(
     void *stream) {
     (void)workspace; (void)workspace_bytes;
     const int32_t st = baracuda_kernels_moe_w4_grouped_gfx950_can_implement(num_experts, topk, size_m, n, k, element, gated);
-    if (st != kOk || size_m == 0) return st;
-    if (!x || !packed || !sorted_token_ids || !expert_ids || !out || !expert_counts || !expert_offsets) return kInvalid;
+    if (st != kOk) return st;
+    if (!expert_counts || !expert_offsets) return kInvalid;
+    if (size_m == 0) {      // no pair, but the counts are filled
+        hipLaunchKernelGGL(moe_offsets_kernel, dim3(1), dim3(1024), 0, (hipStream_t)stream, nullptr, 0, num_experts, expert_counts,
+                           expert_offsets);
+        return launch_status();
+    }
+    if (!x || !packed || !sorted_token_ids || !expert_ids || !out) return kInvalid;
     if ((uintptr_t)x % 16 || (uintptr_t)packed % 16 || (uintptr_t)out % 2 || (uintptr_t)bias % 4 || (uintptr_t)topk_weights % 4)
         return kMisaligned;
     const int32_t in_div = topk_weights ? 1 : topk;

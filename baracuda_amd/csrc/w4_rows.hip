@@ -120,9 +120,9 @@ __global__ __launch_bounds__(64 * WAVES) void rows_kernel(const ProductArgs a) {
     __syncthreads();
     const int ncols = GATED ? a.N / 2 : a.N;
     constexpr int OUT = GATED ? CB / 2 : CB;
-    if (wave < OUT) {
-        const int c = wave * (GATED ? 2 : 1);
-        v4f y = part[c * 64 + lane], u;
+    for (int o = wave; o < OUT; o += WAVES) {
+        const int c = o * (GATED ? 2 : 1);
+        v4f y = part[c * 64 + lane];
 #pragma unroll
         for (int v = 1; v < WAVES; ++v) y += part[(v * CB + c) * 64 + lane];
         int in, out;
@@ -130,21 +130,20 @@ __global__ __launch_bounds__(64 * WAVES) void rows_kernel(const ProductArgs a) {
         int n = 0;
 #pragma unroll
         for (int q = 0; q < CB; ++q) n = q == c ? 16 * row16[q] + 4 * kq : n;
-        if (out >= 0 && n < ncols) {
-            y += bias4(a, w.e, n);
-            if constexpr (GATED) {
-                u = part[(c + 1) * 64 + lane];
+        if (out < 0 || n >= ncols) continue;
+        y += bias4(a, w.e, n);
+        if constexpr (GATED) {
+            v4f u = part[(c + 1) * 64 + lane];
 #pragma unroll
-                for (int v = 1; v < WAVES; ++v) u += part[(v * CB + c + 1) * 64 + lane];
-                u += bias4(a, w.e, n + a.N / 2);
+            for (int v = 1; v < WAVES; ++v) u += part[(v * CB + c + 1) * 64 + lane];
+            u += bias4(a, w.e, n + a.N / 2);
 #pragma unroll
-                for (int q = 0; q < 4; ++q) y[q] = gated(y[q], u[q]);
-            }
-            if constexpr (MOE) {
-                if (a.topk_weights) y *= a.topk_weights[out];
-            }
-            store4<BF16>(a, out, n, ncols, y);
+            for (int q = 0; q < 4; ++q) y[q] = gated(y[q], u[q]);
         }
+        if constexpr (MOE) {
+            if (a.topk_weights) y *= a.topk_weights[out];
+        }
+        store4<BF16>(a, out, n, ncols, y);
     }
     if constexpr (MOE) {
         if (!a.offsets && blockIdx.x == 0 && blockIdx.y == 0) count_experts(a, (uint32_t *)lds);
@@ -175,8 +174,7 @@ template <bool BF16, bool MOE, bool GATED>
 int32_t launch_all(const ProductArgs &a, hipStream_t stream) {
     const int held = MOE ? moe_rows_held(a.size_m, a.E) : rows_held(a.M);
     const int64_t slots = MOE ? std::min<int64_t>(most_tile_rows(a.size_m, a.E, held), a.size_m) : (a.M + held - 1) / held;
-    const int64_t likely = MOE ? std::max(1, a.size_m / held + std::min(a.E, a.size_m) / 2) : slots;
-    const RowsShape s = rows_shape(held, likely, a.N, a.K, GATED);
+    const RowsShape s = rows_shape(held, MOE ? moe_rows_likely(a.size_m, a.E, held) : slots, a.N, a.K, GATED);
 #define BK_W4_ROWS(CB, WAVES) \
     if (s.blocks == CB && s.waves == WAVES) return launch_shape<BF16, MOE, GATED, CB, WAVES>(a, held, slots, stream);
     if constexpr (!GATED) {

@@ -3,55 +3,66 @@
 #pragma once
 
 #include <algorithm>
+#include <cmath>
 #include <cstdint>
 
 namespace bk {
 namespace w4 {
 
 // ---- tiles -----------------------------------------------------------------------
-// Shapes of w4_tiles.hip: TM rows of x by TN rows of the weights.
-enum TileShape { T_32x64, T_32x128, T_32x128_DEEP, T_64x128, T_64x256, T_128x128, T_128x256, T_192x256, T_256x256, T_COUNT };
+// Shapes of w4_tiles.hip: TM rows of x by TN rows of the weights; of two of the same
+// size the DEEP one has a CU to itself and cuts K over groups of waves.
+enum TileShape {
+    T_32x64, T_32x128, T_32x128_DEEP, T_64x128_DEEP, T_64x256, T_128x128_DEEP, T_128x256_DEEP, T_128x256, T_192x256, T_256x256,
+    T_COUNT
+};
 struct TileCost {
     int tm, tn;
+    int share;      // tiles that share a CU
     float fixed;    // us of a round: launch, first loads, end
     float step;     // us per 64 values of K, a tile alone on its CU and few of them
     float load;     // ... how much more of that where every CU has one
-    float paired;   // us per 64 values of two tiles that share a CU (0: LDS holds one)
+    float shared;   // us per 64 values of as many tiles as share a CU
 };
-// Fitted to every shape's times (us) over 32 to 4097 rows, N = 1024 to 60000, K = 512 to
-// 14336, bf16, weights from HBM: the picks lie 0.4% above the best of the nine on the
-// average of 86 sizes, 8% at most.  200 x 11008 x 4096: 128x128 28.7, 64x256 30.9, 64x128
-// 37.4, 128x256 44.3; 777 x 11008 x 4096: 192x256 74.7, 256x256 82.7, 128x128 88.4; 64 x
-// 14336 x 4096: 32x128 deep 15.9, 32x64 18.3, 64x128 20.1; 32 x 60000 x 1024: 32x128 13.2,
-// 64x256 15.1, 32x64 16.9.
+// Fitted to every shape's times (us) over 102 sizes of 32 to 4097 rows, N = 1000 to 60000,
+// K = 512 to 14336, and 70 mixtures, bf16, weights from HBM: the picks lie 0.7% above the
+// best of the ten on the average, 15% at most (of mixtures, whose counts the host does
+// not know, 3.0%).  200 x 11008 x 4096: 128x128 29, 64x256 35, 128x256 44; 777 x 11007 x
+// 4096: 192x256 73, 256x256 82, 128x256 85; 64 x 14336 x 4096: 32x128 deep 15.6, 32x64 18;
+// 64 x 60000 x 1024: 64x256 14, 32x128 19, 128x256 18.
 constexpr TileCost kTileCost[T_COUNT] = {
-    {32, 64, 4.8f, 0.097f, 0.21f, 0.167f},  {32, 128, 4.9f, 0.181f, 0.19f, 0.288f}, {32, 128, 5.4f, 0.132f, 0.07f, 0.0f},
-    {64, 128, 6.2f, 0.187f, 0.26f, 0.0f},   {64, 256, 7.0f, 0.305f, 0.45f, 0.0f},   {128, 128, 5.7f, 0.324f, 0.26f, 0.0f},
-    {128, 256, 7.2f, 0.482f, 0.56f, 0.0f},  {192, 256, 6.2f, 0.882f, 0.25f, 0.0f},  {256, 256, 6.5f, 0.986f, 0.41f, 0.0f},
+    {32, 64, 2, 5.6f, 0.082f, 0.36f, 0.158f},  {32, 128, 3, 6.0f, 0.138f, 0.49f, 0.377f}, {32, 128, 1, 6.0f, 0.132f, 0.0f, 0.0f},
+    {64, 128, 1, 7.0f, 0.176f, 0.27f, 0.0f},   {64, 256, 2, 6.7f, 0.376f, 0.27f, 0.812f}, {128, 128, 1, 6.7f, 0.304f, 0.28f, 0.0f},
+    {128, 256, 1, 9.2f, 0.468f, 0.50f, 0.0f},  {128, 256, 2, 7.9f, 0.449f, 0.78f, 1.362f}, {192, 256, 1, 8.2f, 0.862f, 0.19f, 0.0f},
+    {256, 256, 1, 8.5f, 1.035f, 0.29f, 0.0f},
 };
 constexpr int64_t kMaxTiles = 1 << 22;      // workgroups of a launch
 
-// Of one matrix's rows: up to three rounds of tiles over the 256 CUs are whole ones,
-// later ones overlap.
-inline float tile_us(const TileCost &c, int64_t tiles, int k) {
-    const float kt = (float)((k + 63) / 64), full = (float)tiles / 256.0f;
-    const int64_t rounds = (tiles + 255) / 256;
-    const float one = c.fixed + kt * c.step * (1.0f + c.load * std::min(1.0f, full));
-    if (c.paired == 0.0f) return rounds <= 3 ? (float)rounds * one : (full + 0.5f) * one;
-    const float two = c.fixed + kt * c.paired;
-    return rounds <= 3 ? (float)(rounds / 2) * two + (float)(rounds % 2) * one : (full + 0.5f) / 2.0f * two;
+// n tiles a CU, of a launch that fills `full` of the 256 CUs' first tiles.
+inline float cu_us(const TileCost &c, float n, float full, int k) {
+    const float kt = (float)((k + 63) / 64), one = c.fixed + kt * c.step * (1.0f + c.load * std::min(1.0f, full));
+    if (c.share == 1) return n * one;
+    const float all = c.fixed + kt * c.shared, share = (float)c.share;
+    if (n <= 1.0f) return one;
+    return n <= share ? one + std::max(0.0f, all - one) * (n - 1.0f) / (share - 1.0f) : n / share * all;
 }
 
-// By expert, where the GPU alone knows the counts: an expert's last tile is taken as
-// filled by a third, and a round that may just be passed as half begun.  The picks lie
-// 1.6% above the best shape on the average of 75 mixtures of 2 to 128 experts with uneven
-// shares (with the last tile half full and whole rounds 3.3%).
+// Of one matrix's rows: up to three rounds of tiles over the CUs are whole ones, later
+// ones overlap.
+inline float tile_us(const TileCost &c, int64_t tiles, int k) {
+    const float full = (float)tiles / 256.0f;
+    const int64_t rounds = (tiles + 255) / 256;
+    return cu_us(c, rounds <= 3 * c.share ? (float)rounds : full + 0.5f, full, k);
+}
+
+// By expert, where the GPU alone knows the counts: the experts that can have rows are
+// taken to have them with an exponential spread, and a round that may just be passed as
+// begun.
 inline float moe_tile_us(const TileCost &c, int64_t pairs, int experts, int n, int k) {
-    const float rows = std::max(1.0f, (float)pairs / (float)c.tm + 0.7f * (float)std::min<int64_t>(experts, pairs));
-    const float kt = (float)((k + 63) / 64), full = rows * (float)((n + c.tn - 1) / c.tn) / 256.0f;
-    const float one = c.fixed + kt * c.step * (1.0f + c.load * std::min(1.0f, full)), rounds = std::max(1.0f, full + 0.5f);
-    if (c.paired == 0.0f) return rounds * one;
-    return rounds <= 1.0f ? one : std::max(one, rounds / 2.0f * (c.fixed + kt * c.paired));
+    const float active = (float)std::min<int64_t>(experts, pairs), mean = (float)pairs / active;
+    const float rows = active / (1.0f - std::exp(-0.85f * (float)c.tm / mean));
+    const float full = rows * (float)((n + c.tn - 1) / c.tn) / 256.0f;
+    return cu_us(c, std::max(1.0f, full + (c.share == 1 ? 0.25f : 0.5f)), full, k);
 }
 
 // Tiles of rows that there can be at most.  experts: 0 where the rows are one matrix's.
@@ -101,6 +112,11 @@ inline int rows_held(int64_t rows) { return rows <= 2 ? 2 : rows <= 4 ? 4 : rows
 inline int moe_rows_held(int64_t pairs, int experts) {
     const int most = rows_held(pairs);
     return 4 * pairs < 11 * std::min<int64_t>(experts, pairs) ? std::min(most, 8) : most;
+}
+
+// ... and how many workgroups over the rows are likely.
+inline int64_t moe_rows_likely(int64_t pairs, int experts, int held) {
+    return std::max<int64_t>(1, pairs / held + std::min<int64_t>(experts, pairs) / 2);
 }
 
 struct RowsShape {

@@ -46,9 +46,7 @@ struct Tile {
     static constexpr int NB = TN / 32;                  // blocks of weight rows
     // DMAs a wave and stage: of x (8 rows by 64 values), codes (a tile) and scales (a
     // block's words, of up to four tiles each; with more waves than blocks some are
-    // fetched again, since waves that all do the same meet the barrier together: 256 x
-    // 256 tiles, scales by two of the eight waves, 16 bytes a lane, 810 us in place of
-    // 772 at 4097 x 28672 x 4096)
+    // fetched again: every wave does the same, and none is waited for at the barrier)
     static constexpr int NX = TM / 8 / GROUP, NC = NB / GROUP, NS = (NB + WAVES - 1) / WAVES, NI = NX + NC + NS;
     static constexpr int SUB = TM * 128 + NB * 1024, SCALES = KG * SUB, STAGE = SCALES + NB * 256;
     static constexpr int LDS = DEPTH * STAGE + TM * 4;  // and the output rows
@@ -140,9 +138,12 @@ __device__ __forceinline__ void multiply(Source<T> &src, int K, v16f (&acc)[T::T
                     acc[i][j] = mfma32x32x16<BF16>(wf, xf[h][i], acc[i][j]);
                     const int t = (h * 2 + j) * T::TI + i;
                     if (t % EVERY == 0 && t / EVERY < T::NI) {
-                        __builtin_amdgcn_sched_barrier(0);
+                        // (pinned for small tiles: 128 x 4096 x 4096 11.3 us, else 11.9; large
+                        // ones are better off with the compiler's order: 777 x 11008 x 4096
+                        // 74.6, pinned 76.8)
+                        if constexpr (T::TI == 1) __builtin_amdgcn_sched_barrier(0);
                         src.piece(t / EVERY, nxt, s + T::DEPTH - 1);
-                        __builtin_amdgcn_sched_barrier(0);
+                        if constexpr (T::TI == 1) __builtin_amdgcn_sched_barrier(0);
                     }
                 }
             }
@@ -332,12 +333,13 @@ template <bool BF16, bool MOE, bool GATED>
 int32_t launch_all(const ProductArgs &a, hipStream_t stream) {
     switch (tile_shape(a.size_m, MOE ? a.E : 0, a.N, a.K)) {
         case T_32x64: return launch_tile<BF16, MOE, GATED, Tile<32, 64, 1, 4, 3>>(a, stream);
-        case T_32x128: return launch_tile<BF16, MOE, GATED, Tile<32, 128, 1, 2, 4>>(a, stream);
+        case T_32x128: return launch_tile<BF16, MOE, GATED, Tile<32, 128, 1, 2, 3>>(a, stream);
         case T_32x128_DEEP: return launch_tile<BF16, MOE, GATED, Tile<32, 128, 1, 4, 4>>(a, stream);
-        case T_64x128: return launch_tile<BF16, MOE, GATED, Tile<64, 128, 2, 4, 3>>(a, stream);
-        case T_64x256: return launch_tile<BF16, MOE, GATED, Tile<64, 256, 2, 2, 4>>(a, stream);
-        case T_128x128: return launch_tile<BF16, MOE, GATED, Tile<128, 128, 2, 2, 3>>(a, stream);
-        case T_128x256: return launch_tile<BF16, MOE, GATED, Tile<128, 256, 2, 2, 3>>(a, stream);
+        case T_64x128_DEEP: return launch_tile<BF16, MOE, GATED, Tile<64, 128, 2, 4, 3>>(a, stream);
+        case T_64x256: return launch_tile<BF16, MOE, GATED, Tile<64, 256, 2, 1, 3>>(a, stream);
+        case T_128x128_DEEP: return launch_tile<BF16, MOE, GATED, Tile<128, 128, 2, 2, 3>>(a, stream);
+        case T_128x256_DEEP: return launch_tile<BF16, MOE, GATED, Tile<128, 256, 2, 2, 3>>(a, stream);
+        case T_128x256: return launch_tile<BF16, MOE, GATED, Tile<128, 256, 2, 1, 3>>(a, stream);
         case T_192x256: return launch_tile<BF16, MOE, GATED, Tile<192, 256, 2, 1, 4>>(a, stream);
         default: return launch_tile<BF16, MOE, GATED, Tile<256, 256, 2, 1, 3>>(a, stream);
     }

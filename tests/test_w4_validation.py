@@ -117,6 +117,7 @@ def test_c_entries_refuse():
                        (dict(m=-1), 2), (dict(k=63), 3), (dict(gated=1, n=32), 3)):
         assert linear(**kw) == status, kw
     assert linear(m=0) == 0
+    assert linear(ldx=2 ** 23) == 3 and linear(ldx=2 ** 40) == 3                # a tile of x past 31 bits
     assert L.w4_pack_gfx950_run(1, 32, 32, p, p, p + 4, None) == 1
     assert L.w4_pack_gfx950_run(1, 32, 32, None, p, p, None) == 2
     assert L.w4_pack_gfx950_run(0, 32, 32, None, None, None, None) == 0
@@ -124,9 +125,10 @@ def test_c_entries_refuse():
     assert L.w4_read_gfx950_run(1, 32, 32, 2, p, p, 0, 31, None) == 2
     assert L.w4_quantize_gfx950_run(1, 32, 32, 0, p + 2, 0, 32, p, None) == 1
     moe = L.moe_w4_grouped_gfx950_run
-    assert moe(4, 2, 0, 64, 64, 2, 0, *(None,) * 9, None, 0, None) == 0
+    assert moe(4, 2, 0, 64, 64, 2, 0, *(None,) * 9, None, 0, None) == 2          # nowhere to put the counts
     assert moe(4, 2, 4, 64, 64, 2, 0, p, p, p, None, None, None, p, p, p, None, 0, None) == 2
     assert moe(4, 2, 4, 64, 64, 2, 0, p + 2, p, p, p, None, None, p, p, p, None, 0, None) == 1
+    assert moe(4, 1, 2 ** 20, 64, 4096, 2, 0, p, p, p, p, None, None, p, p, p, None, 0, None) == 3      # x past 31 bits
 
 
 @pytest.mark.parametrize("n,k", [(1, 32), (32, 128), (33, 96), (64, 256), (100, 288), (4096, 4096)])
