@@ -74,8 +74,8 @@ __device__ __forceinline__ int expert_tiles(const ProductArgs &a) {
     return __builtin_amdgcn_readfirstlane(n);
 }
 
-// The same for at most kFewPairs pairs from the ids themselves, which
-// saves the launch in front that counts them.
+// expert_rows for at most kFewPairs pairs, from the ids themselves: that saves the
+// launch in front that counts them (about 3 us of a step of 30).
 constexpr int kFewPairs = 256;
 template <int TB>
 __device__ __forceinline__ bool expert_rows_few(const ProductArgs &a, int slot, Rows &r) {

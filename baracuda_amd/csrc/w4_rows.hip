@@ -14,9 +14,15 @@ namespace {
 // tiles), and the same values of x's row l % 16.  Gated: odd blocks are rows of the
 // second half of the matrix, whose products meet those of the first half in the same
 // lanes.  A wave takes a word (256 values of K, four tiles) at a time: codes and
-// scales into registers, x by LDS DMA into 512 bytes a row of its own, 16-byte unit u
-// of row r at u ^ (r & 15), two buffers; the next word's are asked for before this
-// one's are waited for.
+// scales into registers, the next word's asked for before this one is multiplied; x by
+// LDS DMA into 512 bytes a row of its own, 16-byte unit u of row r at u ^ (r & 15).
+// (Straight from L2 into registers a row's 64 bytes at a time x bounded it: 16 x 4096 x
+// 4096 7.5 us, now 5.8; 16 x 28672 x 4096 20 and 17.  A second buffer of x costs more in
+// workgroups that fit a CU than it hides: 16 x 14336 x 4096 11.0 and 10.5.)
+//
+// The weights' bytes bound it, behind a launch and one round trip of 2.4 us: one row of
+// 131072 x 16384 moves them at 6.0 TB/s, 28672 x 4096 in 13.8 us (4.5), 4096 x 4096 in
+// 3.5 to 4.4.
 template <bool BF16, bool MOE, bool GATED, int HELD, int CB, int WAVES>
 __global__ __launch_bounds__(64 * WAVES) void rows_kernel(const ProductArgs a) {
     extern __shared__ __attribute__((aligned(1024))) int8_t lds[];
@@ -58,8 +64,8 @@ __global__ __launch_bounds__(64 * WAVES) void rows_kernel(const ProductArgs a) {
             r.scale[c] = *(const uint32_t *)(scales[c] + (int64_t)s * 256);
         }
     };
-    // x: HELD rows a buffer, two a DMA; rows that there are not and values past K lie past
-    // the extent and land as zeros
+    // x: up to HELD rows, two a DMA; rows that there are not and values past K lie past the
+    // extent and land as zeros
     int8_t *own = lds + wave * (HELD * 512);
     const v4i rsrc = MOE ? mfma2::make_rsrc(a.x, (uint32_t)((int64_t)((a.size_m + a.in_div - 1) / a.in_div) * a.K * 2))
                          : mfma2::make_rsrc(a.x + w.first * a.ldx, (uint32_t)(((w.rows - 1) * a.ldx + a.K) * 2));

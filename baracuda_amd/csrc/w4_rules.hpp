@@ -36,7 +36,7 @@ constexpr TileCost kTileCost[T_COUNT] = {
     {128, 256, 1, 9.2f, 0.468f, 0.50f, 0.0f},  {128, 256, 2, 7.9f, 0.449f, 0.78f, 1.362f}, {192, 256, 1, 8.2f, 0.862f, 0.19f, 0.0f},
     {256, 256, 1, 8.5f, 1.035f, 0.29f, 0.0f},
 };
-constexpr int64_t kMaxTiles = 1 << 22;      // workgroups of a launch
+constexpr int64_t kMaxTiles = 1 << 21;      // workgroups of a launch, of up to 1024 threads
 
 // n tiles a CU, of a launch that fills `full` of the 256 CUs' first tiles.
 inline float cu_us(const TileCost &c, float n, float full, int k) {

@@ -689,7 +689,7 @@ int32_t baracuda_kernels_kv_pages_gfx950_can_implement(int32_t layers, int64_t n
  * Lane l of tile t holds row 32 b + l % 32, values 64 t + 32 (l / 32) .. + 31, two
  * codes a byte, the lower index in the lower four bits; byte j of a lane's scales is
  * that of tile 4 s + j.  Rows past N and values past K are zeros.  Several matrices
- * lie one after the other. */
+ * lie one after the other.  Outputs overlap no input. */
 size_t baracuda_kernels_w4_packed_bytes_gfx950(int32_t n, int32_t k);
 
 /* Weights [matrices, N, K] (strides in elements, K dense) to packed ones: the scale
@@ -725,7 +725,7 @@ size_t baracuda_kernels_w4_linear_gfx950_workspace_size(int32_t m, int32_t n, in
  * out[id] = end(x[row] W_e^T + bias[e]) [* topk_weights[id]], rounded once.  x has
  * ceil(size_m / topk) rows (size_m when topk_weights != NULL), packed [E] matrices,
  * bias f32 [E, N] or NULL.  expert_counts [E] and expert_offsets [E + 1] are filled by
- * the call.  Positions whose expert is num_experts or more, all of them last, and ids
+ * the call (calls at the same time need their own).  Positions whose expert is num_experts or more, all of them last, and ids
  * outside the pairs are left out: nothing is written for them. */
 int32_t baracuda_kernels_moe_w4_grouped_gfx950_run(
     int32_t num_experts, int32_t topk, int32_t size_m, int32_t n, int32_t k, int32_t element, int32_t gated, const void *x,

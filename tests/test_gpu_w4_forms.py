@@ -95,3 +95,38 @@ def test_two_streams_at_once(gpu):
     for x, out in zip(xs, outs):
         ok, why = plain.close(out, *plain.product(x, plain.values(codes, scales)[0]))
         assert ok, why
+
+
+def test_output_past_32_bits(gpu):
+    """More than 2^31 elements of output; the last rows are the last rows' product."""
+    from baracuda_amd import w4
+    from tests.test_gpu_w4 import _gen, _packed, _randn
+    m, n, k, g = 66001, 33000, 32, _gen(5)
+    codes, scales = plain.checkpoint(g, 1, n, k)
+    x = _randn(g, m, k).to(BF)
+    out = torch.empty(m, n, dtype=BF, device=gpu)
+    w4.W4LinearPlan.select(w4.W4LinearDescriptor(m, n, k)).run(x, _packed(codes, scales), out)
+    for rows in (slice(0, 3), slice(m // 2, m // 2 + 3), slice(m - 40, m)):
+        ok, why = plain.close(out[rows], *plain.product(x[rows], plain.values(codes, scales)[0]))
+        assert ok, why
+
+
+@pytest.mark.parametrize("pairs", [3, 400])
+def test_weights_past_32_bits(gpu, pairs):
+    """An expert that lies behind 4 GiB of others."""
+    from baracuda_amd import w4
+    from tests.test_gpu_w4 import _gen, _packed, _randn
+    e, n, k, g = 3, 131072, 32768, _gen(6)
+    codes, scales = plain.checkpoint(g, e, n, k)
+    packed = _packed(codes, scales)
+    assert 2 * packed.shape[1] > 2 ** 32
+    x = _randn(g, pairs, k).to(BF)
+    i32 = dict(dtype=torch.int32, device=gpu)
+    ids = torch.full((pairs,), 2, **i32)
+    out = torch.empty(pairs, n, dtype=BF, device=gpu)
+    w4.MoeW4GroupedPlan.select(w4.MoeW4GroupedDescriptor(e, 1, pairs, n, k)).run(
+        x, packed, torch.arange(pairs, **i32), ids, out, torch.empty(e, **i32), torch.empty(e + 1, **i32))
+    for rows in (slice(0, 50), slice(n - 50, n)):
+        want, error = plain.product(x, plain.values(codes[2, rows], scales[2, rows]))
+        ok, why = plain.close(out[:, rows], want, error)
+        assert ok, why

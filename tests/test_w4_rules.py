@@ -83,7 +83,7 @@ def test_forms_are_all_there_are(rules):
         for rows, e in ((m, 0), (pairs, experts)):
             form = _moe(rules, rows, e, n, k, gated) if e else _linear(rules, rows, n, k, gated)
             if form[0] == "tile":
-                assert rules.workgroups(form[1], rows, e, n) <= 1 << 22
+                assert rules.workgroups(form[1], rows, e, n) <= 1 << 21
             else:
                 assert -(-rows // form[1]) + min(e, rows) <= 65535
     assert found["linear"] <= set(w4_forms.LINEAR)
