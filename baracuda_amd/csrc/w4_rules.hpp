@@ -27,7 +27,7 @@ struct TileCost {
 // Fitted to every shape's times (us) over 102 sizes of 32 to 4097 rows, N = 1000 to 60000,
 // K = 512 to 14336, and 70 mixtures, bf16, weights from HBM: the picks lie 0.7% above the
 // best of the ten on the average, 15% at most (of mixtures, whose counts the host does
-// not know, 3.0%).  200 x 11008 x 4096: 128x128 29, 64x256 35, 128x256 44; 777 x 11007 x
+// not know, 1.4%).  200 x 11008 x 4096: 128x128 29, 64x256 35, 128x256 44; 777 x 11007 x
 // 4096: 192x256 73, 256x256 82, 128x256 85; 64 x 14336 x 4096: 32x128 deep 15.6, 32x64 18;
 // 64 x 60000 x 1024: 64x256 14, 32x128 19, 128x256 18.
 constexpr TileCost kTileCost[T_COUNT] = {
@@ -56,13 +56,14 @@ inline float tile_us(const TileCost &c, int64_t tiles, int k) {
 }
 
 // By expert, where the GPU alone knows the counts: the experts that can have rows are
-// taken to have them with an exponential spread, and a round that may just be passed as
-// begun.
+// taken to have them with an exponential spread, tiles of rows in whole numbers.  Tiles
+// that share CUs overlap their rounds, and half of one more is taken as begun.
 inline float moe_tile_us(const TileCost &c, int64_t pairs, int experts, int n, int k) {
     const float active = (float)std::min<int64_t>(experts, pairs), mean = (float)pairs / active;
-    const float rows = active / (1.0f - std::exp(-0.85f * (float)c.tm / mean));
+    const float rows = std::max(1.0f, std::round(active / (1.0f - std::exp(-0.85f * (float)c.tm / mean))));
     const float full = rows * (float)((n + c.tn - 1) / c.tn) / 256.0f;
-    return cu_us(c, std::max(1.0f, full + (c.share == 1 ? 0.25f : 0.5f)), full, k);
+    const float rounds = c.share == 1 && full <= 2.5f ? std::ceil(full) : full + 0.5f;
+    return cu_us(c, std::max(1.0f, rounds), full, k);
 }
 
 // Tiles of rows that there can be at most.  experts: 0 where the rows are one matrix's.
