@@ -102,7 +102,7 @@ int32_t baracuda_kernels_moe_w4_grouped_gfx950_run(
     ProductArgs a{};
     a.x = (const uint16_t *)x, a.w = (const uint8_t *)packed, a.bias = bias, a.out = (uint16_t *)out;
     a.ldx = k, a.ldo = gated ? n / 2 : n;
-    const bool rows = moe_rows_pay(size_m, num_experts, n), few = rows && size_m <= kFewPairs, bf16 = element == kv4::kBf16;
+    const bool rows = moe_rows_pay(size_m, num_experts, n), few = size_m <= kFewPairs, bf16 = element == kv4::kBf16;
     a.order = sorted_token_ids, a.expert_ids = expert_ids, a.topk_weights = topk_weights;
     a.offsets = few ? nullptr : expert_offsets, a.counts_out = expert_counts, a.offsets_out = expert_offsets;
     a.E = num_experts, a.size_m = size_m, a.in_div = in_div;

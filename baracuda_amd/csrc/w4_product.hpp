@@ -60,7 +60,7 @@ __device__ __forceinline__ bool expert_rows(const ProductArgs &a, int slot, Rows
     return false;
 }
 
-// Tiles of TB rows in all, as every lane's value.
+// Tiles of TB rows in all.
 template <int TB>
 __device__ __forceinline__ int expert_tiles(const ProductArgs &a) {
     const int lane = threadIdx.x & 63;
@@ -75,10 +75,11 @@ __device__ __forceinline__ int expert_tiles(const ProductArgs &a) {
 }
 
 // expert_rows for at most kFewPairs pairs, from the ids themselves: that saves the
-// launch in front that counts them (about 3 us of a step of 30).
+// launch in front that counts them (about 3 us of a step of 30).  Past the list `slot`
+// is left smaller by the list's length.
 constexpr int kFewPairs = 256;
 template <int TB>
-__device__ __forceinline__ bool expert_rows_few(const ProductArgs &a, int slot, Rows &r) {
+__device__ __forceinline__ bool expert_rows_few(const ProductArgs &a, int &slot, Rows &r) {
     constexpr int CHUNKS = kFewPairs / 64;
     const int lane = threadIdx.x & 63;
     int id[CHUNKS];
@@ -112,6 +113,14 @@ __device__ __forceinline__ bool expert_rows_few(const ProductArgs &a, int slot, 
         if (head[i]) from = 64 * i + 63 - __clzll((long long)head[i]);
     }
     return false;
+}
+
+template <int TB>
+__device__ __forceinline__ int expert_tiles_few(const ProductArgs &a) {
+    int left = INT32_MAX;
+    Rows none;
+    expert_rows_few<TB>(a, left, none);
+    return INT32_MAX - left;
 }
 
 // expert_counts and expert_offsets of few pairs, by one whole workgroup, through

@@ -29,7 +29,8 @@ __global__ __launch_bounds__(64 * WAVES) void rows_kernel(const ProductArgs a) {
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     Rows w;
     if constexpr (MOE) {
-        if (!(a.offsets ? expert_rows<HELD>(a, blockIdx.y, w) : expert_rows_few<HELD>(a, blockIdx.y, w))) {     // the whole workgroup
+        int slot = blockIdx.y;
+        if (!(a.offsets ? expert_rows<HELD>(a, slot, w) : expert_rows_few<HELD>(a, slot, w))) {     // the whole workgroup
             if (!a.offsets && blockIdx.x == 0 && blockIdx.y == 0) count_experts(a, (uint32_t *)lds);
             return;
         }

@@ -275,7 +275,13 @@ __global__ __launch_bounds__(64 * T::WAVES) void tiles_kernel(const ProductArgs 
     int tm, tn;
     Rows w;
     if constexpr (MOE) {
-        if (!tile_of(expert_tiles<T::TM>(a), tiles_n, tm, tn) || !expert_rows<T::TM>(a, tm, w)) return;
+        if (!a.offsets && blockIdx.x == 0) {
+            count_experts(a, (uint32_t *)lds);
+            __syncthreads();
+        }
+        if (!tile_of(a.offsets ? expert_tiles<T::TM>(a) : expert_tiles_few<T::TM>(a), tiles_n, tm, tn)) return;
+        int slot = tm;
+        if (!(a.offsets ? expert_rows<T::TM>(a, slot, w) : expert_rows_few<T::TM>(a, slot, w))) return;
     } else {
         if (!tile_of((a.M + T::TM - 1) / T::TM, tiles_n, tm, tn)) return;
         w = Rows{0, tm * T::TM, min(T::TM, a.M - tm * T::TM)};

@@ -60,6 +60,11 @@ def test_few_pairs_found_from_the_ids(gpu, experts, pairs):
     one = [0] * (experts - 1) + [pairs]
     ok, why = plain.close(*_grouped(one, 33, 96, BF, False, 1, False, False, seed=experts))
     assert ok, why
+    if experts < 50:      # wide enough for tiles
+        ok, why = plain.close(*_grouped(counts, 4161, 96, BF, False, 1, False, True, seed=experts, none=min(3, 256 - pairs)))
+        assert ok, why
+        ok, why = plain.close(*_grouped(one, 4224, 160, F16, True, 1, True, False, seed=experts))
+        assert ok, why
 
 
 @pytest.mark.parametrize("m", [0, 1])

@@ -67,6 +67,11 @@ def test_cases_take_their_forms(rules):
         assert _moe(rules, pairs, experts, n, k, gated) == form, (pairs, experts, n, k, gated)
 
 
+@pytest.mark.parametrize("experts,pairs", [(3, 65), (5, 64), (9, 256), (2, 200), (7, 63)])
+def test_few_pairs_of_wide_experts_take_tiles(rules, experts, pairs):
+    assert _moe(rules, pairs, experts, 4161, 96, False)[0] == _moe(rules, pairs, experts, 4224, 160, True)[0] == "tile"
+
+
 def test_forms_are_all_there_are(rules):
     """No sizes take a form that the cases lack, and none of the launches is too large."""
     rng = random.Random(1)
