@@ -13,7 +13,7 @@ constexpr int kMaxExperts = 1024;
 // equal ids: the first lane of each run adds the run's length to the expert's
 // LDS counter (any order of the ids counts right; ids outside [0, E) nowhere),
 // and the counts' prefix sum runs over the 16 waves.  One ballot per expert
-// and 64 ids, and the sum by one thread, took 29 us at 3072 ids of 64 experts
+// and 64 ids, and the sum by one thread, took 29 us at the ids of 512 tokens, 6 of 64 experts,
 // and 7.7 at 8192 of 8; now 4.6 and 5.7.
 __global__ __launch_bounds__(1024) void moe_offsets_kernel(const int32_t *__restrict__ expert_ids,
                                                            int size_m, int num_experts,

@@ -5,7 +5,9 @@
 // of scales a lane, 4352 bytes) through LDS: on the matrix's side a wave touches
 // whole rows of 256 columns, on the packed side the piece's 4 KiB of codes are
 // contiguous.  Nothing is computed but the group's largest magnitude and the
-// hardware's conversions, so the float side's bytes bound them.
+// hardware's conversions, so the float side's bytes bound them: 8 x 14336 x 4096 f32
+// weights (1.9 GB) quantized in 413 us, 5.2 TB/s, read back in 475, 4.5; a large copy
+// moves 5.0.  bf16 4096 x 4096: 8.5 and 8.0 us.
 #include "w4.hpp"
 
 namespace bk {
