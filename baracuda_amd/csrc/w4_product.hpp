@@ -77,40 +77,33 @@ __device__ __forceinline__ int expert_tiles(const ProductArgs &a) {
 // expert_rows for at most kFewPairs pairs, from the ids themselves: that saves the
 // launch in front that counts them (about 3 us of a step of 30).  Past the list `slot`
 // is left smaller by the list's length.
-constexpr int kFewPairs = 256;
 template <int TB>
 __device__ __forceinline__ bool expert_rows_few(const ProductArgs &a, int &slot, Rows &r) {
-    constexpr int CHUNKS = kFewPairs / 64;
     const int lane = threadIdx.x & 63;
-    int id[CHUNKS];
-    uint64_t head[CHUNKS];                 // positions whose expert is not the one before
+    int id[kFewChunks];
+    uint64_t head[kFewChunks];             // positions whose expert is not the one before
 #pragma unroll
-    for (int i = 0; i < CHUNKS; ++i) id[i] = 64 * i + lane < a.size_m ? a.expert_ids[64 * i + lane] : -1;
+    for (int i = 0; i < kFewChunks; ++i) id[i] = 64 * i + lane < a.size_m ? a.expert_ids[64 * i + lane] : -1;
 #pragma unroll
-    for (int i = 0; i < CHUNKS; ++i) {
+    for (int i = 0; i < kFewChunks; ++i) {
         const int before = i ? __builtin_amdgcn_readlane(id[i ? i - 1 : 0], 63) : -2, up = __shfl_up(id[i], 1, 64);
         head[i] = __ballot(id[i] != (lane ? up : before));
     }
     int from = 0;                          // where the run that reaches into this chunk began
 #pragma unroll
-    for (int i = 0; i < CHUNKS; ++i) {
-        const uint64_t upto = head[i] & (~0ull >> (63 - lane));
-        const int began = upto ? 64 * i + 63 - __clzll((long long)upto) : from;
-        const uint64_t starts = __ballot((unsigned)id[i] < (unsigned)a.E && (64 * i + lane - began) % TB == 0);
+    for (int i = 0; i < kFewChunks; ++i) {
+        const uint64_t starts = __ballot((unsigned)id[i] < (unsigned)a.E && (64 * i + lane - run_began(head[i], i, lane, from)) % TB == 0);
         const int n = __popcll(starts);
         if (slot < n) {
             const bool me = (starts >> lane & 1) && __popcll(starts & ((1ull << lane) - 1)) == slot;
             const int l = __builtin_amdgcn_readfirstlane(__ffsll((unsigned long long)__ballot(me)) - 1);
             r.e = __builtin_amdgcn_readlane(id[i], l);
             r.first = 64 * i + l;
-            const uint64_t later = l < 63 ? head[i] >> (l + 1) : 0, next = i + 1 < CHUNKS ? head[i + 1 < CHUNKS ? i + 1 : 0] : 1;
-            // a run of more than TB goes on in another tile, so what lies in the next chunk is enough
-            const int run = later ? __ffsll((unsigned long long)later) : 64 - l + (next ? __ffsll((unsigned long long)next) - 1 : 64);
-            r.rows = min(min(TB, run), a.size_m - r.first);
+            r.rows = min(min(TB, run_left<TB>(head, i, l)), a.size_m - r.first);
             return true;
         }
         slot -= n;
-        if (head[i]) from = 64 * i + 63 - __clzll((long long)head[i]);
+        from = run_began(head[i], i, 63, from);
     }
     return false;
 }

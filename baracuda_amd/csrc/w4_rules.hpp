@@ -120,6 +120,38 @@ inline int64_t moe_rows_likely(int64_t pairs, int experts, int held) {
     return std::max<int64_t>(1, pairs / held + std::min<int64_t>(experts, pairs) / 2);
 }
 
+// ---- few pairs of a mixture --------------------------------------------------------
+// Up to this many sorted pairs a workgroup finds its expert's rows from the ids, 64
+// positions (a chunk) at a time: bit l of head[i] is set where position 64 i + l has
+// another id than the one before it, as the first position past the pairs has.
+constexpr int kFewPairs = 256, kFewChunks = kFewPairs / 64;
+
+// Where the run of equal ids began that holds position 64 i + l; `from`: the run that
+// reaches into chunk i.
+constexpr int run_began(uint64_t head, int i, int l, int from) {
+    const uint64_t upto = head & (~0ull >> (63 - l));
+    return upto ? 64 * i + 63 - __builtin_clzll(upto) : from;
+}
+
+// Positions of that run from 64 i + l on; where there are TB of them or more, TB or more.
+// TB rows from any lane touch REACH chunks behind their own at most.
+template <int TB>
+constexpr int run_left(const uint64_t (&head)[kFewChunks], int i, int l) {
+    constexpr int REACH = (TB + 62) / 64;
+    const uint64_t later = l < 63 ? head[i] >> (l + 1) : 0;
+    if (later) return __builtin_ctzll(later) + 1;
+    int left = 64 - l;
+#if defined(__clang__)
+#pragma unroll
+#endif
+    for (int j = 1; j <= REACH; ++j) {
+        if (i + j >= kFewChunks) break;
+        if (head[i + j]) return left + __builtin_ctzll(head[i + j]);
+        left += 64;
+    }
+    return left;
+}
+
 struct RowsShape {
     int blocks, waves;      // of 16 weight rows a workgroup; that divide K
 };
