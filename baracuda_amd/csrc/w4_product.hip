@@ -22,6 +22,9 @@ bool too_many(int64_t rows, int32_t experts, int32_t n) {
 // Byte offsets of x within a tile, or of all rows that pairs name, fit 31 bits.
 bool extent_ok(int64_t rows, int64_t ld, int32_t k) { return ((rows - 1) * ld + k) * 2 < mfma2::kPastExtent; }
 
+// Rows of x that pairs name, in_div pairs a row.
+int64_t x_rows(int32_t size_m, int32_t in_div) { return ((int64_t)size_m + in_div - 1) / in_div; }
+
 void sizes(ProductArgs &a, int32_t n, int32_t k) {
     a.N = n, a.K = k, a.tiles = tiles(k), a.words = scale_words(k), a.matrix = matrix_bytes(n, k);
 }
@@ -71,6 +74,8 @@ int32_t baracuda_kernels_moe_w4_grouped_gfx950_can_implement(int32_t num_experts
     const int32_t st = product_ok(n, k, element, gated);
     if (st != kOk) return st;
     if (num_experts > kMaxExperts || size_m > (1 << 20) || too_many(size_m, num_experts, n)) return kUnsupported;
+    // with router weights x has a row for each pair, which `run` alone can tell
+    if (size_m > 0 && !extent_ok(x_rows(size_m, topk), k, k)) return kUnsupported;
     return kOk;
 }
 
@@ -98,7 +103,7 @@ int32_t baracuda_kernels_moe_w4_grouped_gfx950_run(
     if ((uintptr_t)x % 16 || (uintptr_t)packed % 16 || (uintptr_t)out % 2 || (uintptr_t)bias % 4 || (uintptr_t)topk_weights % 4)
         return kMisaligned;
     const int32_t in_div = topk_weights ? 1 : topk;
-    if (!extent_ok((size_m + in_div - 1) / in_div, k, k)) return kUnsupported;
+    if (!extent_ok(x_rows(size_m, in_div), k, k)) return kUnsupported;
     ProductArgs a{};
     a.x = (const uint16_t *)x, a.w = (const uint8_t *)packed, a.bias = bias, a.out = (uint16_t *)out;
     a.ldx = k, a.ldo = gated ? n / 2 : n;

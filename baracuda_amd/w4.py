@@ -168,7 +168,11 @@ class MoeW4GroupedPlan:
     ``plans.MoeS8GroupedPlan``: position p of the pairs sorted by expert is pair
     sorted_token_ids[p] of expert expert_ids[p]; a pair's input row is pair / topk
     (the pair's own with topk_weights, which scale its output), its output row the
-    pair's own.  Positions of no expert (num_experts, all of them last) are left out."""
+    pair's own.  Positions of no expert (num_experts, all of them last) are left out.
+
+    The rows of x times K are less than 2^30.  ``select`` refuses what passes it with
+    ceil(size_m / topk) rows; with topk_weights x has size_m rows, and ``run`` refuses
+    those that pass it."""
 
     def __init__(self, desc: MoeW4GroupedDescriptor):
         d = self.desc = desc

@@ -712,7 +712,8 @@ int32_t baracuda_kernels_w4_weights_gfx950_can_implement(int32_t matrices, int32
  * f16 or bf16; sums, bias and gate in 32 bits, rounded once.  Weights enter as
  * elements: exactly in bf16 for scales of 2^-125 to 2^125, in f16 for scales of 2^-23
  * to 2^13, beyond that rounded to the element.  x is 16-byte aligned, ldx a multiple
- * of 8. */
+ * of 8.  M is at most 2^20, N 2^24, K 2^22 and N K 2^36 (can_implement), and with more
+ * than one row 255 ldx + K is less than 2^30 - 8 (run). */
 int32_t baracuda_kernels_w4_linear_gfx950_run(int32_t m, int32_t n, int32_t k, int32_t element, int32_t gated, const void *x,
                                               int64_t ldx, const void *packed, const float *bias, void *out, int64_t ldo,
                                               void *workspace, size_t workspace_bytes, void *stream);
@@ -725,8 +726,11 @@ size_t baracuda_kernels_w4_linear_gfx950_workspace_size(int32_t m, int32_t n, in
  * out[id] = end(x[row] W_e^T + bias[e]) [* topk_weights[id]], rounded once.  x has
  * ceil(size_m / topk) rows (size_m when topk_weights != NULL), packed [E] matrices,
  * bias f32 [E, N] or NULL.  expert_counts [E] and expert_offsets [E + 1] are filled by
- * the call (calls at the same time need their own).  Positions whose expert is num_experts or more, all of them last, and ids
- * outside the pairs are left out: nothing is written for them. */
+ * the call (calls at the same time need their own).  Positions whose expert is
+ * num_experts or more, all of them last, and ids outside the pairs are left out:
+ * nothing is written for them.  At most 1024 experts and 2^20 pairs, and the rows of x
+ * times K are less than 2^30: of ceil(size_m / topk) rows can_implement decides it, of
+ * the size_m rows that x has with topk_weights `run` does. */
 int32_t baracuda_kernels_moe_w4_grouped_gfx950_run(
     int32_t num_experts, int32_t topk, int32_t size_m, int32_t n, int32_t k, int32_t element, int32_t gated, const void *x,
     const void *packed, const int32_t *sorted_token_ids, const int32_t *expert_ids, const float *topk_weights,
