@@ -9,7 +9,9 @@
 //   scales  [ceil(N / 32)][ceil(K / 256)][64][4]
 // bytes.  Lane l of a tile is row l % 32 of its block of rows and group l / 32 of
 // the tile's two, 16 bytes with the lower index in the lower four bits; byte j of
-// a lane's four scales is that of tile 4 s + j.  What lies past N or K is zero.
+// a lane's four scales is that of tile 4 s + j.  Past N or K codes are 0 and scale bytes
+// 2.  (The products multiply weights by zeros of x there, also those of other tiles under
+// such a byte, so that it has to leave them finite: 0 does as well, 255 does not.)
 // So a tile is one kilobyte that a wave reads in one piece, 16 bytes a lane, and
 // what a lane gets are the words of the matrix operands that it supplies: row l %
 // 32 and eight values of K a word for the 32x32x16 product, or, from two tiles,

@@ -688,8 +688,9 @@ int32_t baracuda_kernels_kv_pages_gfx950_can_implement(int32_t layers, int64_t n
  *   scales  [ceil(N / 32)][ceil(K / 256)][64][4]
  * Lane l of tile t holds row 32 b + l % 32, values 64 t + 32 (l / 32) .. + 31, two
  * codes a byte, the lower index in the lower four bits; byte j of a lane's scales is
- * that of tile 4 s + j.  Rows past N and values past K are zeros.  Several matrices
- * lie one after the other.  Outputs overlap no input. */
+ * that of tile 4 s + j.  For rows past N and values past K codes are 0 and scale bytes
+ * 2 (or 0; never 255 or another that makes a weight infinite: it would reach the
+ * results as NaN).  Several matrices lie one after the other.  Outputs overlap no input. */
 size_t baracuda_kernels_w4_packed_bytes_gfx950(int32_t n, int32_t k);
 
 /* Weights [matrices, N, K] (strides in elements, K dense) to packed ones: the scale
