@@ -302,10 +302,15 @@ __global__ __launch_bounds__(64 * T::WAVES) void tiles_kernel(const ProductArgs 
         const int block = __builtin_amdgcn_readfirstlane(block_of((wave * T::NC + j) % T::NB));
         src.codes[j] = mfma2::make_rsrc(matrix + (int64_t)block * a.tiles * 1024, block < blocks ? a.tiles * 1024 : 0);
     }
-    // (a block past the last takes whatever follows, for columns that are not stored)
-    src.scales = mfma2::make_rsrc(matrix + (int64_t)blocks * a.tiles * 1024, (uint32_t)a.words * blocks * 256);
+    // The scales from the tile's first block on: a matrix may have more than 2^31 bytes of
+    // them, of which the blocks of one tile span half and a little at most (gated).  (A block
+    // past the last takes whatever follows, for columns that are not stored.)
+    const int first = block_of(0);
+    src.scales = mfma2::make_rsrc(matrix + (int64_t)blocks * a.tiles * 1024 + (int64_t)first * a.words * 256,
+                                  (uint32_t)a.words * (uint32_t)(blocks - first) * 256);
 #pragma unroll
-    for (int j = 0; j < T::NS; ++j) src.word[j] = __builtin_amdgcn_readfirstlane(block_of((wave * T::NS + j) % T::NB)) * a.words * 256;
+    for (int j = 0; j < T::NS; ++j)
+        src.word[j] = __builtin_amdgcn_readfirstlane((block_of((wave * T::NS + j) % T::NB) - first) * a.words * 256);
     if constexpr (MOE) {
         const int x_rows = (a.size_m + a.in_div - 1) / a.in_div;
         src.x = mfma2::make_rsrc(a.x, (uint32_t)((int64_t)x_rows * a.K * 2));

@@ -29,3 +29,33 @@ def test_padding_scales_of_zero(gpu, dtype, m, n, k):
     assert torch.equal(*outs)
     ok, why = plain.close(outs[1], *plain.product(x, plain.values(codes, scales)[0]))
     assert ok, why
+
+
+@pytest.mark.parametrize("m,gated", [(1, False), (17, False), (17, True)])
+def test_scales_past_31_bits(gpu, m, gated):
+    """More than 2^31 bytes of scales: weights are zero but in a few blocks of 32 rows, the
+    first and last of them and those where the scales pass 2^31."""
+    n, k, g = 16646592, 4128, _gen(m)
+    blocks, codes_of, scales_of = n // 32, -(-k // 128) * 2048, -(-k // 256) * 256
+    assert blocks * scales_of > 2 ** 31 and n * k <= 2 ** 36
+    edge = 2 ** 31 // scales_of
+    some = [0, 1, blocks // 2 - 1, blocks // 2, blocks // 2 + 1, edge - 1, edge, edge + 1, blocks - 2, blocks - 1]
+    codes, scales = plain.checkpoint(g, 1, 32 * len(some), k)
+    part = _packed(codes, scales)[0]
+    packed = torch.zeros(w4.packed_bytes(n, k), dtype=torch.uint8, device=gpu)
+    c, s = packed[:blocks * codes_of].view(blocks, -1), packed[blocks * codes_of:].view(blocks, -1)
+    at = torch.tensor(some, device=gpu)
+    c[at], s[at] = part[:len(some) * codes_of].view(len(some), -1), part[len(some) * codes_of:].view(len(some), -1)
+    x = _randn(g, m, k).to(BF)
+    out = torch.full((m, n // 2 if gated else n), 3.0, dtype=BF, device=gpu)
+    w4.W4LinearPlan.select(w4.W4LinearDescriptor(m, n, k, gated=gated)).run(x, packed, out)
+    w = dict(zip(some, plain.values(codes, scales)[0].view(len(some), 32, k)))
+    none = torch.zeros(32, k, dtype=torch.float64, device=gpu)
+    half = blocks // 2
+    for b in sorted({b % half if gated else b for b in some} | {5, half - 3}):
+        rows = torch.cat((w.get(b, none), w.get(b + half, none))) if gated else w.get(b, none)
+        ok, why = plain.close(out[:, 32 * b:32 * b + 32], *plain.product(x, rows, None, gated))
+        assert ok, (b, why)
+    written = torch.zeros(out.shape[1] // 32, dtype=torch.bool, device=gpu)
+    written[torch.tensor([b % half if gated else b for b in some], device=gpu)] = True
+    assert not bool(out.view(m, -1, 32)[:, ~written].any())
