@@ -167,13 +167,25 @@ int32_t launch_held(const ProductArgs &a, int64_t slots, hipStream_t stream) {
     return launch_status();
 }
 
-template <bool BF16, bool MOE, bool GATED, int CB, int WAVES>
-int32_t launch_shape(const ProductArgs &a, int held, int64_t slots, hipStream_t stream) {
-    switch (held) {
-        case 2: return launch_held<BF16, MOE, GATED, 2, CB, WAVES>(a, slots, stream);
-        case 4: return launch_held<BF16, MOE, GATED, 4, CB, WAVES>(a, slots, stream);
-        case 8: return launch_held<BF16, MOE, GATED, 8, CB, WAVES>(a, slots, stream);
-        default: return launch_held<BF16, MOE, GATED, 16, CB, WAVES>(a, slots, stream);
+template <bool BF16, bool MOE, bool GATED, int HELD, int CB>
+int32_t launch_blocks(const ProductArgs &a, int waves, int64_t slots, hipStream_t stream) {
+#define BK_W4_WAVES(WAVES)                          \
+    if constexpr (rows_form(HELD, CB, WAVES, GATED)) \
+        if (waves == WAVES) return launch_held<BF16, MOE, GATED, HELD, CB, WAVES>(a, slots, stream);
+    BK_W4_WAVES(2)
+    BK_W4_WAVES(4)
+    BK_W4_WAVES(8)
+    BK_W4_WAVES(16)
+#undef BK_W4_WAVES
+    return kUnsupported;
+}
+
+template <bool BF16, bool MOE, bool GATED, int HELD>
+int32_t launch_shape(const ProductArgs &a, const RowsShape &s, int64_t slots, hipStream_t stream) {
+    switch (s.blocks) {
+        case 1: return launch_blocks<BF16, MOE, GATED, HELD, 1>(a, s.waves, slots, stream);
+        case 2: return launch_blocks<BF16, MOE, GATED, HELD, 2>(a, s.waves, slots, stream);
+        default: return launch_blocks<BF16, MOE, GATED, HELD, 4>(a, s.waves, slots, stream);
     }
 }
 
@@ -182,22 +194,12 @@ int32_t launch_all(const ProductArgs &a, hipStream_t stream) {
     const int held = MOE ? moe_rows_held(a.size_m, a.E) : rows_held(a.M);
     const int64_t slots = MOE ? std::min<int64_t>(most_tile_rows(a.size_m, a.E, held), a.size_m) : (a.M + held - 1) / held;
     const RowsShape s = rows_shape(held, MOE ? moe_rows_likely(a.size_m, a.E, held) : slots, a.N, a.K, GATED);
-#define BK_W4_ROWS(CB, WAVES) \
-    if (s.blocks == CB && s.waves == WAVES) return launch_shape<BF16, MOE, GATED, CB, WAVES>(a, held, slots, stream);
-    if constexpr (!GATED) {
-        BK_W4_ROWS(1, 4)
-        BK_W4_ROWS(1, 8)
-        BK_W4_ROWS(1, 16)
+    switch (held) {
+        case 2: return launch_shape<BF16, MOE, GATED, 2>(a, s, slots, stream);
+        case 4: return launch_shape<BF16, MOE, GATED, 4>(a, s, slots, stream);
+        case 8: return launch_shape<BF16, MOE, GATED, 8>(a, s, slots, stream);
+        default: return launch_shape<BF16, MOE, GATED, 16>(a, s, slots, stream);
     }
-    BK_W4_ROWS(2, 2)
-    BK_W4_ROWS(2, 4)
-    BK_W4_ROWS(2, 8)
-    BK_W4_ROWS(2, 16)
-    BK_W4_ROWS(4, 2)
-    BK_W4_ROWS(4, 4)
-    BK_W4_ROWS(4, 8)
-#undef BK_W4_ROWS
-    return kUnsupported;
 }
 
 }  // namespace

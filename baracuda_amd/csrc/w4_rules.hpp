@@ -180,5 +180,16 @@ inline RowsShape rows_shape(int held, int64_t slots, int n, int k, bool gated) {
     return s;
 }
 
+// Whether rows_shape gives this form for any sizes, so that no other is compiled: one or
+// two blocks for up to 2 rows held, no four for up to 4; two waves for two blocks or more
+// on 512 workgroups, which 16 rows held by two blocks never have; sixteen for fewer blocks
+// than four.
+constexpr bool rows_form(int held, int blocks, int waves, bool gated) {
+    if (blocks == 1 ? gated : blocks == 2 ? held == 2 && !gated : held <= 4) return false;
+    if (waves == 2) return blocks == 4 || (blocks == 2 && held < 16);
+    return waves == 16 ? blocks < 4 : waves == 4 || waves == 8;
+}
+
+
 }  // namespace w4
 }  // namespace bk
