@@ -102,7 +102,8 @@ class W4WeightsPlan:
 
     def pack(self, codes, scales, packed, stream=None) -> None:
         """From codes uint8 [.., N, K / 2] and scales uint8 [.., N, K / 32], as a
-        checkpoint holds them; the descriptor's element has no part in it."""
+        checkpoint holds them; the descriptor's element has no part in it, and no scale is
+        refused: what a product's element cannot hold is rounded there (W4LinearPlan)."""
         st = _w4.pack(self._packed, stream, codes, scales, packed)
         if st:
             check(st, "W4WeightsPlan::pack")
@@ -126,7 +127,10 @@ class W4LinearDescriptor:
 
 class W4LinearPlan:
     """out [M, N] (gated: [M, N / 2]) = x [M, K] W^T + bias, f32 [N].  Sums, bias and
-    gate are held in 32 bits and rounded once."""
+    gate are held in 32 bits and rounded once.  Weights enter as elements: in bf16 as
+    they are (scales of 2^-125 to 2^125), in f16 with scales of 2^-23 to 2^13; beyond
+    these they are rounded to the element, in f16 to infinity from 65520 on.  ``quantize``
+    keeps scales of f16 weights below that, a checkpoint in bf16 or f32 need not."""
 
     def __init__(self, desc: W4LinearDescriptor):
         d = self.desc = desc

@@ -59,3 +59,26 @@ def test_scales_past_31_bits(gpu, m, gated):
     written = torch.zeros(out.shape[1] // 32, dtype=torch.bool, device=gpu)
     written[torch.tensor([b % half if gated else b for b in some], device=gpu)] = True
     assert not bool(out.view(m, -1, 32)[:, ~written].any())
+
+
+@pytest.mark.parametrize("dtype", [BF, F16], ids=str)
+@pytest.mark.parametrize("m", [1, 3, 16, 20, 90, 300])
+def test_every_scale_rounds_to_the_element(gpu, dtype, m):
+    """Scales beyond those with which weights are elements, one of 256 a row: a weight enters
+    as its value rounded to the element, infinite past its range.  x is one power of two
+    and zeros, so that each result is one product, rounded once."""
+    n, k, g = 256, 32, _gen(m)
+    some = torch.randint(0, 256, (1, n, k // 2), generator=g, device=gpu, dtype=torch.uint8)
+    scales = torch.arange(256, device=gpu).to(torch.uint8).view(1, n, 1).contiguous()
+    plan = w4.W4LinearPlan.select(w4.W4LinearDescriptor(m, n, k, element=KIND[dtype]))
+    for power in (-14, 0, 12) if dtype == F16 else (-40, 0, 20):
+        for at in (0, 7, 31):
+            codes = torch.zeros_like(some)                  # no zero of x meets an infinity
+            codes[..., at // 2] = some[..., at // 2] & (0xf0 if at % 2 else 0x0f)
+            x = torch.zeros(m, k, dtype=dtype, device=gpu)
+            x[:, at] = 2.0 ** power
+            out = torch.zeros(m, n, dtype=dtype, device=gpu)
+            plan.run(x, _packed(codes, scales), out)
+            w = plain.values(codes, scales)[0, :, at].to(dtype).double()
+            want = (w * 2.0 ** power).to(dtype).expand(m, n)
+            assert bool(((out == want) | (out.isnan() & want.isnan())).all()), (power, at)
