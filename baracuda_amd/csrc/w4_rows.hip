@@ -18,7 +18,9 @@ namespace {
 // LDS DMA into 512 bytes a row of its own, 16-byte unit u of row r at u ^ (r & 15).
 // (Straight from L2 into registers a row's 64 bytes at a time x bounded it: 16 x 4096 x
 // 4096 7.5 us, now 5.8; 16 x 28672 x 4096 20 and 17.  A second buffer of x costs more in
-// workgroups that fit a CU than it hides: 16 x 14336 x 4096 11.0 and 10.5.)
+// workgroups that fit a CU than it hides: 16 x 14336 x 4096 11.0 and 10.5.  x and the weights are
+// waited for together, so that a wave has one word of them in flight; an earlier form with
+// x in registers took 12.5 us for one row of 28672 x 4096 gated, this one 13.9.)
 //
 // The weights' bytes bound it, behind a launch and one round trip of 2.4 us: one row of
 // 131072 x 16384 moves them at 6.0 TB/s, 28672 x 4096 in 13.8 us (4.5), 4096 x 4096 in

@@ -163,7 +163,9 @@ struct RowsShape {
 // Waves: eight, sixteen for a deep K on a small grid (1 x 4096 x 14336 8.2, with eight
 // 10.5), four on a large grid of wide workgroups (16 x 28672 x 4096 17.1, 18.5) and for up
 // to four words of K (1 x 60000 x 1024 8.4, 10.7), two of both (16 x 60000 x 1024 10.6, with
-// four 12.1).
+// four 12.1).  Gated, sixteen waves spill 20 to 24 registers at the end and pay on the
+// smallest grids alone: 1 x 1024 x 14336 10.4, with eight 12.3, 1 x 2048 x 8192 7.9 / 8.2, but
+// 1 x 4096 x 8192 9.0 / 8.9, 1 x 7168 x 8192 10.9 / 10.4, 8 x 7168 x 8192 11.7 / 11.0.
 inline RowsShape rows_shape(int held, int64_t slots, int n, int k, bool gated) {
     const int64_t g = (int64_t)((n + 15) / 16) * slots;
     const int words = (k + 255) / 256;

@@ -11,10 +11,11 @@
 // group l / 32 of its tile, word i of its 16 bytes the eight values of product i;
 // x's operand takes the same eight values, 16-byte unit 4 (l / 32) + i of its row.
 //
-// Large tiles are bound by the board's power (4097 x 28672 x 4096: 1240 TFLOP/s, 65% of
-// the matrix unit's clocks at 1.75 GHz; with x's DMA left out 10% faster), tiles of few
-// rows by the DMA of x, 26 clocks a kilobyte of a CU, and by a tile's first loads and end,
-// 5 to 8 us, which tiles that share a CU hide from one another.
+// Large tiles are bound by the board's power: 4097 x 28672 x 4096 gated, by tiles of
+// 128x256, two a CU, 1210 to 1310 TFLOP/s at 1.68 GHz with 73% of the matrix unit's clocks
+// busy (without the gate 1.6 and 76%).  Tiles of few rows are bound by the DMA of x, 26
+// clocks a kilobyte of a CU, and by a tile's first loads and end, 5 to 8 us, which tiles
+// that share a CU hide from one another.
 #include "gemm_mfma2.hpp"
 #include "w4_product.hpp"
 
