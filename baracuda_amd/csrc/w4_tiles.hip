@@ -306,12 +306,12 @@ __global__ __launch_bounds__(64 * T::WAVES) void tiles_kernel(const ProductArgs 
     // The scales from the tile's first block on: a matrix may have more than 2^31 bytes of
     // them, of which the blocks of one tile span half and a little at most (gated).  (A block
     // past the last takes whatever follows, for columns that are not stored.)
-    const int first = block_of(0);
-    src.scales = mfma2::make_rsrc(matrix + (int64_t)blocks * a.tiles * 1024 + (int64_t)first * a.words * 256,
-                                  (uint32_t)a.words * (uint32_t)(blocks - first) * 256);
+    const int first = __builtin_amdgcn_readfirstlane(block_of(0)), block_scales = a.words * 256;
+    src.scales = mfma2::make_rsrc(matrix + (int64_t)blocks * a.tiles * 1024 + (int64_t)first * block_scales,
+                                  (uint32_t)(blocks - first) * (uint32_t)block_scales);
 #pragma unroll
     for (int j = 0; j < T::NS; ++j)
-        src.word[j] = __builtin_amdgcn_readfirstlane((block_of((wave * T::NS + j) % T::NB) - first) * a.words * 256);
+        src.word[j] = (__builtin_amdgcn_readfirstlane(block_of((wave * T::NS + j) % T::NB)) - first) * block_scales;
     if constexpr (MOE) {
         const int x_rows = (a.size_m + a.in_div - 1) / a.in_div;
         src.x = mfma2::make_rsrc(a.x, (uint32_t)((int64_t)x_rows * a.K * 2));
